@@ -19,7 +19,7 @@ LIB = os.path.join(HERE, "libssattn.so")
 # measurement build: the same sources with the router's phase stamps and the
 # attention kernel's step stamps compiled in
 STAMPS_LIB = os.path.join(HERE, "libssattn_stamps.so")
-SOURCES = ("attention.hip", "route.hip", "pset.hip", "summary.hip", "runtime.hip", "group.hip")
+SOURCES = ("attention.hip", "route.hip", "pset.hip", "summary.hip", "runtime.hip", "group.hip", "append.hip", "paged.hip")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
          # packed fp32 VALU forms are excluded from code generation
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -28,7 +28,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
 # (their inputs are finite), so max/min of matrix-pipe results need no
 # signalling-NaN quieting; pset.hip keeps IEEE NaN semantics (it tests scores
 # for finiteness).
-EXTRA = {"attention.hip": ["-fno-honor-nans"], "route.hip": ["-fno-honor-nans"]}
+EXTRA = {"attention.hip": ["-fno-honor-nans"], "route.hip": ["-fno-honor-nans"], "paged.hip": ["-fno-honor-nans"]}
 NOISE = "is not a recognized feature for this target"
 
 
