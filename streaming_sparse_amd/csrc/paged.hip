@@ -19,6 +19,9 @@
 #include "../../include/ssattn_paged.h"
 
 #include <algorithm>
+#include <array>
+#include <cmath>
+#include <type_traits>
 
 using namespace ssa;
 
@@ -42,17 +45,19 @@ struct PagedParams {
   float* part;
   int tokens, batch, per_seq, heads, kv_heads, group, pages, prefix_tokens, table_pages, causal;
   float scale_log2;
-  int row_tiles;      // 32-row tiles of a K/V head's rows: the states' layout
-  // Work items of the launch, prefix items first: prefix_tiles tiles per K/V
-  // head (of all sequences' rows), each in prefix_pieces pieces; then
-  // own_tiles tiles per K/V head (of one sequence's rows) in own_pieces pieces,
-  // which walk the prefix too where there are no prefix items.
-  int prefix_tiles, prefix_pieces, own_tiles, own_pieces;
+  // Work items of the launch: prefix_items of the prefix by itself
+  // (prefix_tiles tiles per K/V head, of all sequences' rows, each in
+  // prefix_pieces pieces), then those of the sequences: own_tiles tiles per K/V
+  // head, the first own_whole of all heads' whole, the others in own_pieces
+  // pieces.  They walk the prefix too unless it is `apart`.
+  int prefix_items, prefix_tiles, prefix_pieces, own_tiles, own_whole, own_pieces, apart;
+  int row_tiles;      // 32-row tiles of a K/V head's rows, where the prefix is apart
 };
 
-// A piece's state of 32 rows: O [dim / 4][row] of 4 floats (dim / 4 = 8 dt + 2 j
-// + hh), m [32], l [32].  Piece c of K/V head h, rows 32 T .. at ((c * kv_heads +
-// h) * row_tiles + T) * kState.
+// A piece's state of 32 rows: O [dim / 4][row] of 4 floats, m [32], l [32].  Where
+// the prefix is apart, rows keep their places: piece c of K/V head h, rows 32 T ..
+// at ((c * kv_heads + h) * row_tiles + T) * kState, the prefix's pieces first.
+// Otherwise the tiles behind own_whole have theirs, piece by piece.
 constexpr int kState = 32 * kHeadDim + 64;
 
 template <bool F16>
@@ -106,19 +111,25 @@ __device__ __forceinline__ int vswz(int row) { return (0xEA40 >> (4 * (row & 3))
 
 __device__ __forceinline__ float max3f(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
 
-// Maximum of a lane's 16 scores and its other half's (lane ^ 32: the other keys
-// of the same row).
-__device__ __forceinline__ float row_max(const f32x16& S) {
+// Maximum of a lane's 16 scores, and of both lanes that hold a row (l, l ^ 32).
+template <typename V>
+__device__ __forceinline__ float lane_max(const V& S) {
   const float a = max3f(S[0], S[1], S[2]), b = max3f(S[3], S[4], S[5]), c = max3f(S[6], S[7], S[8]);
   const float d = max3f(S[9], S[10], S[11]), e = max3f(S[12], S[13], S[14]);
-  const float mx = __builtin_fmaxf(max3f(a, b, c), max3f(d, e, S[15]));
-  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+  return __builtin_fmaxf(max3f(a, b, c), max3f(d, e, S[15]));
+}
+__device__ __forceinline__ float half_max(float x) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
 }
 
 __device__ __forceinline__ float half_sum(float x) {
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+}
+
+__device__ __forceinline__ float lse_of(float M, float l) {
+  return __float_as_uint(l) == 0u ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 __device__ __forceinline__ u32x4 tr_pair(const lds_u8* a, const lds_u8* b) {
@@ -131,7 +142,8 @@ __device__ __forceinline__ u32x4 tr_pair(const lds_u8* a, const lds_u8* b) {
 struct Job {
   int h;              // K/V head
   int rho0, rho1;     // rows
-  int piece, pieces, state;   // this piece of the list; the state index it is written to, -1: out
+  int piece, pieces;  // this piece of the list
+  int state;          // where its states go, -1: it writes out
   int b, n, length, first_token;   // the rows' sequence: new tokens, rows in the cache, first packed token
   int prefix_pages, own_pages;     // pages of the list
 };
@@ -178,44 +190,71 @@ __device__ __forceinline__ int packed_tokens(const PagedParams& p) {
   return p.starts ? clampi(p.starts[p.batch], 0, p.tokens) : p.tokens;
 }
 
-// The job of work item `item` for tiles of T rows; false: nothing to do.
+// The rows of the idx-th own tile of T rows over all K/V heads; false: none.
 template <int T>
-__device__ __forceinline__ bool find_job(const PagedParams& p, int item, int lane, Job& j) {
-  const int prefix_items = p.kv_heads * p.prefix_tiles * p.prefix_pieces;
-  const int all_prefix = (p.prefix_tokens + kPage - 1) / kPage;
-  j.b = -1;
-  j.n = j.length = j.first_token = 0;
-  if (item < prefix_items) {
-    const int tp = item / p.prefix_pieces;
-    j.piece = item - tp * p.prefix_pieces;
-    j.h = tp / p.prefix_tiles;
-    j.rho0 = (tp - j.h * p.prefix_tiles) * T;
-    j.rho1 = min(j.rho0 + T, packed_tokens(p) * p.group);
-    j.pieces = p.prefix_pieces;
-    j.state = j.piece;
-    j.prefix_pages = all_prefix;
-    j.own_pages = 0;
-    return j.rho0 < j.rho1;
-  }
-  const int tp = (item - prefix_items) / p.own_pieces;
-  j.piece = item - prefix_items - tp * p.own_pieces;
-  j.h = tp / p.own_tiles;
-  const SeqTile s = find_tile(p, tp - j.h * p.own_tiles, T, lane);
+__device__ __forceinline__ bool find_rows(const PagedParams& p, int idx, int lane, Job& j) {
+  j.h = idx / p.own_tiles;
+  const SeqTile s = find_tile(p, idx - j.h * p.own_tiles, T, lane);
   if (s.b < 0) return false;
   j.b = s.b;
   j.n = s.n;
   j.first_token = s.start;
-  j.length = clampi(p.lengths[s.b], 0, kPage * p.table_pages);
   j.rho0 = s.start * p.group + s.tile * T;
   j.rho1 = min(j.rho0 + T, (s.start + s.n) * p.group);
-  j.pieces = p.own_pieces;
-  j.state = prefix_items || p.own_pieces > 1 ? p.prefix_pieces + j.piece : -1;
-  j.prefix_pages = prefix_items ? 0 : all_prefix;
+  return j.rho0 < j.rho1;
+}
+
+// Prefix item `item` of tiles of T rows; false: no rows.
+template <int T>
+__device__ __forceinline__ bool prefix_job(const PagedParams& p, int item, Job& j) {
+  const int tp = item / p.prefix_pieces;
+  j.piece = item - tp * p.prefix_pieces;
+  j.h = tp / p.prefix_tiles;
+  j.rho0 = (tp - j.h * p.prefix_tiles) * T;
+  j.rho1 = min(j.rho0 + T, packed_tokens(p) * p.group);
+  j.pieces = p.prefix_pieces;
+  j.state = j.piece;
+  j.b = 0;
+  j.n = j.length = j.first_token = 0;
+  j.prefix_pages = (p.prefix_tokens + kPage - 1) / kPage;
+  j.own_pages = 0;
+  return j.rho0 < j.rho1;
+}
+
+// Own item `item` (behind the prefix items) of tiles of T rows; false: no rows.
+template <int T>
+__device__ __forceinline__ bool own_job(const PagedParams& p, int item, int lane, Job& j) {
+  int tile = item;
+  j.piece = 0;
+  j.pieces = 1;
+  j.state = p.apart ? p.prefix_pieces : -1;
+  if (item >= p.own_whole) {
+    const int i = item - p.own_whole, t = i / p.own_pieces;
+    j.piece = i - t * p.own_pieces;
+    j.pieces = p.own_pieces;
+    j.state = p.apart ? p.prefix_pieces + j.piece : p.own_pieces > 1 ? i : -1;
+    tile = p.own_whole + t;
+  }
+  if (!find_rows<T>(p, tile, lane, j)) return false;
+  j.length = clampi(p.lengths[j.b], 0, kPage * p.table_pages);
+  j.prefix_pages = p.apart ? 0 : (p.prefix_tokens + kPage - 1) / kPage;
   // rows the tile's last query sees
   int seen = j.length;
   if (p.causal) seen = clampi(j.length - j.n + (j.rho1 - 1) / p.group - j.first_token + 1, 0, j.length);
   j.own_pages = (seen + kPage - 1) / kPage;
-  return j.rho0 < j.rho1;
+  return true;
+}
+
+// The state that holds row rho (block `blk` of a tile of T rows) of a job, and
+// its place in it.
+template <int T>
+__device__ __forceinline__ float* state_of(const PagedParams& p, const Job& j, int rho, int blk, int* col) {
+  if (p.apart) {
+    *col = rho & 31;
+    return p.part + (((long long)j.state * p.kv_heads + j.h) * p.row_tiles + (rho >> 5)) * kState;
+  }
+  *col = (rho - j.rho0) & 31;
+  return p.part + ((long long)j.state * (T / 32) + blk) * kState;
 }
 
 // The pages of a job's list, walked upwards: lane l holds page base + l of the
@@ -230,13 +269,16 @@ struct PageList {
     int id = -1;
     if (u < j.prefix_pages)
       id = p.prefix[u];
-    else if (u < j.prefix_pages + j.own_pages)
+    else if (u - j.prefix_pages < p.table_pages)
       id = p.table[(long long)j.b * p.table_pages + (u - j.prefix_pages)];
     return id >= 0 && id < p.pages ? id : -1;
   }
+  // A list that fits both windows is held from its start, so that its entries
+  // are requested without waiting for the sequence's length.
   __device__ __forceinline__ PageList(const PagedParams& p, const Job& j, int first, int lane)
-      : base(first), cur(fetch(p, j, first + lane)), next(fetch(p, j, first + 64 + lane)) {}
-  // page u of the list; u never decreases by more than the list's base
+      : base(j.prefix_pages + p.table_pages <= 128 ? 0 : first), cur(fetch(p, j, base + lane)),
+        next(fetch(p, j, base + 64 + lane)) {}
+  // page u of the list; u never decreases
   __device__ __forceinline__ Unit at(const PagedParams& p, const Job& j, int u, int lane) {
     if (u - base >= 64) {
       base += 64;
@@ -252,36 +294,80 @@ struct PageList {
 };
 
 // ---------------------------------------------------------------------------
-// Narrow tiles: 32 rows.  Bound by the pages' way from memory, so the four waves
-// of a workgroup walk the list by themselves, 32 keys at a time: wave w takes
-// half pages w, w + 4, ..., its K and V rows going straight to two LDS slots of
-// its own (32 KB a wave) while it computes on the other, with no barrier before
-// the end, where the four states are joined.  The matrix pipe has time to spare:
+// Narrow tiles: 32 rows.  Bound by the pages' way from memory, so waves walk the
+// list by themselves, 32 keys at a time: of the NW waves that share a tile, wave
+// w takes half pages w, w + NW, ..., its K and V rows going straight to 16 KB of
+// LDS of its own, with no barrier before the end, where the states are joined.
+// K of the wave's next half page is requested as soon as the scores are formed,
+// its V as soon as V is read, and eight waves of a CU wait at different times, so
+// that something is always on its way.  The matrix pipe has time to spare:
 // probabilities meet V in two parts (hi + lo), so that no rounding of theirs
 // shows in the output.
 constexpr int kNarrow = 32, kNarrowWaves = 4;
 constexpr int kHalf = 32 * 256;      // 32 rows of K or V
 
-template <bool F16>
-__global__ __launch_bounds__(64 * kNarrowWaves) void narrow_kernel(PagedParams p) {
-  __shared__ alignas(16) uint8_t ring[kNarrowWaves * 4 * kHalf];   // per wave: K, V of slot 0, K, V of slot 1
-  __shared__ float xm[kNarrowWaves][32], xl[kNarrowWaves][32];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  Job j;
-  if (!find_job<kNarrow>(p, xcd_remap(blockIdx.x, gridDim.x), lane, j)) return;
-  const int r = lane & 31, hh = lane >> 5;
-  const int rho = j.rho0 + r;
-  const bool live = rho < j.rho1;
-  const int token = min(rho, j.rho1 - 1) / p.group, hq = j.h * p.group + min(rho, j.rho1 - 1) % p.group;
-  // rows of its sequence that this row sees
-  const int limit = p.causal ? j.length - j.n + (token - j.first_token) + 1 : j.length;
+template <int N>
+__device__ __forceinline__ void loads_left() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
-  // half pages [begin, end) of the list, every fourth from begin + wave
+// Writes what a lane holds of a row: 16 groups of 4 dims (8 c + 4 hh of row
+// rho = j.rho0 + 32 blk + lane % 32), the maximum M and the sum l; to the row's
+// state, or to out and lse.
+template <bool F16, int T>
+__device__ __forceinline__ void finish_row(const PagedParams& p, const Job& j, const f32x16 (&O)[4], float M, float l,
+                                           int blk, int lane) {
+  const int rho = j.rho0 + 32 * blk + (lane & 31), hh = lane >> 5;
+  if (rho >= j.rho1) return;
+  if (j.state >= 0) {
+    int col;
+    float* st = state_of<T>(p, j, rho, blk, &col);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const f32x16& o = O[c >> 2];
+      const int i = 4 * (c & 3);
+      *reinterpret_cast<f32x4*>(st + ((2 * c + hh) * 32 + col) * 4) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+    }
+    if (hh == 0) {
+      st[32 * kHeadDim + col] = M;
+      st[32 * kHeadDim + 32 + col] = l;
+    }
+    return;
+  }
+  const int token = rho / p.group, hq = j.h * p.group + rho % p.group;
+  const bool none = __float_as_uint(l) == 0u;
+  const float inv = none ? 0.0f : 1.0f / l;
+  uint16_t* op = p.out + (long long)token * p.o_tok + (long long)hq * p.o_head + 4 * hh;
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    const f32x16 o = O[c >> 2] * inv;
+    const int i = 4 * (c & 3);
+    *reinterpret_cast<u32x2*>(op + 8 * c) = u32x2{pack2<F16>(o[i], o[i + 1]), pack2<F16>(o[i + 2], o[i + 3])};
+  }
+  if (p.lse && hh == 0) p.lse[(long long)token * p.heads + hq] = lse_of(M, l);
+}
+
+// NW waves share a tile; NW = 1: a wave by itself.
+template <bool F16, int NW>
+__device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
+  const int r = lane & 31, hh = lane >> 5;
+  u32x4 qop[8];
+  int limit;         // rows of its sequence that the lane's row sees
+  {
+    const int rho = min(j.rho0 + r, j.rho1 - 1);
+    const int token = rho / p.group, hq = j.h * p.group + rho % p.group;
+    limit = p.causal ? j.length - j.n + (token - j.first_token) + 1 : j.length;
+    const uint16_t* qp = p.q + (long long)token * p.q_tok + (long long)hq * p.q_head + 8 * hh;
+#pragma unroll
+    for (int st = 0; st < 8; ++st) qop[st] = ldg16(qp + 16 * st);
+  }
+  const int all_see = __builtin_amdgcn_readfirstlane(limit);
+
+  // half pages [begin, end) of the list
   const int units = j.prefix_pages + j.own_pages;
   const int begin = 2 * (int)((long long)units * j.piece / j.pieces);
   const int end = 2 * (int)((long long)units * (j.piece + 1) / j.pieces);
 
-  lds_u8* const base = (lds_u8*)ring + wave * (4 * kHalf);
   // per-lane byte offsets of 16 rows' loads (instruction form: load jj leaves
   // out the 1024 jj that its offset field adds)
   uint32_t koff[4], voff[4];
@@ -295,64 +381,52 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void narrow_kernel(PagedParams p
   const long long rows16 = 32 * p.kv_tok;       // bytes of 16 rows
   const uint8_t* const kh = (const uint8_t*)(p.k + (long long)j.h * p.kv_head);
   const uint8_t* const vh = (const uint8_t*)(p.v + (long long)j.h * p.kv_head);
-  auto issue = [&](const Unit& u, int hu, int slot) {
+  lds_u8* const kb = ring + wave * (2 * kHalf);
+  lds_u8* const vb = kb + kHalf;
+  auto issue = [&](const uint8_t* from, const uint32_t (&off)[4], const Unit& u, int hu, lds_u8* to) {
     // an absent page reads page 0: its rows are masked and its values cleared
     const long long at = (4ll * max(u.page, 0) + 2 * (hu & 1)) * rows16;
-    const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)base + slot * (2 * kHalf));
-    dma_rows<4>(kh + at, koff, l);
-    dma_rows<4>(kh + at + rows16, koff, l + 4096);
-    dma_rows<4>(vh + at, voff, l + kHalf);
-    dma_rows<4>(vh + at + rows16, voff, l + kHalf + 4096);
+    const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)to);
+    dma_rows<4>(from + at, off, l);
+    dma_rows<4>(from + at + rows16, off, l + 4096);
   };
 
   f32x16 O[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
   float m = -INFINITY, ls = 0.0f;
-  int hu = begin + wave;
+  int hu = begin + (NW == 1 ? 0 : wave);
   PageList list(p, j, hu >> 1, lane);
-  Unit u0{-1, 0}, u1{-1, 0};
+  Unit u{-1, 0};
   if (hu < end) {
-    u0 = list.at(p, j, hu >> 1, lane);
-    issue(u0, hu, 0);
-  }
-  if (hu + kNarrowWaves < end) {
-    u1 = list.at(p, j, (hu + kNarrowWaves) >> 1, lane);
-    issue(u1, hu + kNarrowWaves, 1);
-  }
-  u32x4 qop[8];
-  {
-    const uint16_t* qp = p.q + (long long)token * p.q_tok + (long long)hq * p.q_head + 8 * hh;
-#pragma unroll
-    for (int st = 0; st < 8; ++st) qop[st] = ldg16(qp + 16 * st);
+    u = list.at(p, j, hu >> 1, lane);
+    issue(kh, koff, u, hu, kb);
+    issue(vh, voff, u, hu, vb);
   }
   // everything so far, once and in a form the compiler counts: it does not
-  // know of the loads above, and would wait for the query rows in every step
+  // know of the row loads, and would wait for the query rows in every step
   wait_loads();
-  for (int slot = 0; hu < end; hu += kNarrowWaves, slot ^= 1) {
-    const bool more = hu + kNarrowWaves < end;
-    const lds_u8* kb = base + slot * (2 * kHalf);
-    lds_u8* vb = base + slot * (2 * kHalf) + kHalf;
-    // K landed: at most this slot's V and the next slot's 16 loads are out
-    if (more)
-      asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  for (; hu < end; hu += NW) {
+    const bool more = hu + NW < end;
+    loads_left<8>();                                        // K landed, V behind it
     f32x16 S = {};
 #pragma unroll
-    for (int st = 0; st < 8; ++st) {
-      const u32x4 a = *(lds_u32x4*)(kb + r * 256 + (((2 * st + hh) ^ (r & 15)) << 4));
-      S = mma<F16>(a, qop[st], S);
+    for (int st = 0; st < 8; ++st)
+      S = mma<F16>(*(lds_u32x4*)(kb + r * 256 + (((2 * st + hh) ^ (r & 15)) << 4)), qop[st], S);
+    Unit after{-1, 0};
+    if (more) {
+      after = list.at(p, j, (hu + NW) >> 1, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // K is read
+      issue(kh, koff, after, hu + NW, kb);
     }
-    // keys of this half page that the row sees; S[i] is key 8 (i / 4) + 4 hh + i % 4
-    const int rows = u0.rows - 32 * (hu & 1);
-    int see = rows;
-    if ((hu >> 1) >= j.prefix_pages) see = min(see, limit - 32 * (hu - 2 * j.prefix_pages));
-    if (!__all(see >= 32)) {
+    // keys of this half page that a row sees; S[i] is key 8 (i / 4) + 4 hh + i % 4
+    const int rows = u.rows - 32 * (hu & 1), own = hu - 2 * j.prefix_pages;
+    if (min(rows, own >= 0 ? all_see - 32 * own : 32) < 32) {
+      const int see = (own >= 0 ? min(rows, limit - 32 * own) : rows) - 4 * hh;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) S[i] = 8 * (i / 4) + 4 * hh + i % 4 < see ? S[i] : -INFINITY;
+      for (int i = 0; i < 16; ++i) S[i] = 8 * (i / 4) + i % 4 < see ? S[i] : -INFINITY;
     }
-    const float mx = row_max(S) * p.scale_log2;
+    const float mx = half_max(lane_max(S)) * p.scale_log2;
     if (__any(mx > m + kSlack)) {
       const float to = __builtin_fmaxf(m, mx);
       const float a = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));
@@ -362,16 +436,25 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void narrow_kernel(PagedParams p
       m = to;
     }
     const float nb = kLift<F16> - (m == -INFINITY ? 0.0f : m);
-    float P[16];
+    u32x4 hi[2], lo[2];
+    {
+      float P[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      P[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, nb));
-      ls += P[i];
+      for (int i = 0; i < 16; ++i) {
+        P[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, nb));
+        ls += P[i];
+      }
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const u32x2 x = split2<F16>(P[2 * w], P[2 * w + 1]);
+        hi[w >> 2][w & 3] = x[0];
+        lo[w >> 2][w & 3] = x[1];
+      }
     }
     if (more)
-      asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+      loads_left<8>();                                      // V landed, the K just requested behind it
     else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      loads_left<0>();
     if (rows < 32) {
       // rows behind the end hold anything: 0 * NaN must not reach the sums
 #pragma unroll
@@ -380,13 +463,6 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void narrow_kernel(PagedParams p
     }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      u32x4 hi, lo;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const u32x2 x = split2<F16>(P[8 * ks + 2 * w], P[8 * ks + 2 * w + 1]);
-        hi[w] = x[0];
-        lo[w] = x[1];
-      }
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) {
         // dims 32 dt + lane % 32 of keys 16 ks + 8 (e / 4) + 4 hh + e % 4
@@ -394,91 +470,386 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void narrow_kernel(PagedParams p
         const int chunk = 4 * dt + 2 * (g & 1) + ((i & 3) >> 1), row = 16 * ks + 4 * (g >> 1) + (i >> 2);
         const lds_u8* a = vb + row * 256 + ((chunk ^ vswz(row)) << 4) + (i & 1) * 8;
         const u32x4 va = tr_pair(a, a + 2048);
-        O[dt] = mma<F16>(va, hi, O[dt]);
-        O[dt] = mma<F16>(va, lo, O[dt]);
+        O[dt] = mma<F16>(va, hi[ks], O[dt]);
+        O[dt] = mma<F16>(va, lo[ks], O[dt]);
       }
     }
-    // this slot's reads are done before its next rows land
-    u0 = u1;
-    if (hu + 2 * kNarrowWaves < end) {
-      u1 = list.at(p, j, (hu + 2 * kNarrowWaves) >> 1, lane);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      issue(u1, hu + 2 * kNarrowWaves, slot);
+    if (more) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // V is read
+      issue(vh, voff, after, hu + NW, vb);
     }
+    u = after;
   }
 
-  // the four waves' states into one: the sums of a row's two half waves first
+  // the lane's row, formed anew so that no register holds it across the loop
+  int e = lane;
+  asm volatile("" : "+v"(e));
   const float l = half_sum(ls);
   const float mine = m == -INFINITY ? m : m - kLift<F16>;
-  if (hh == 0) {
-    xm[wave][r] = mine;
-    xl[wave][r] = l;
-  }
-  __syncthreads();
-  float M = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kNarrowWaves; ++w) M = __builtin_fmaxf(M, xm[w][r]);
-  const float Mu = M == -INFINITY ? 0.0f : M;
-  float L = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kNarrowWaves; ++w) L += xl[w][r] * __builtin_amdgcn_exp2f(xm[w][r] - Mu);
-  const float a = __builtin_amdgcn_exp2f(mine - Mu);
-  // every wave hands over its 32 x 128 sums, [dim tile][j][lane] of 4 floats,
-  // and adds up one dim tile (the rings are free: all loads have landed)
-  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-  lds_u8* const x = (lds_u8*)ring;
-#pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *(lds_f32x4*)(x + wave * 16384 + (dt * 4 + i) * 1024 + lane * 16) =
-          f32x4{O[dt][4 * i], O[dt][4 * i + 1], O[dt][4 * i + 2], O[dt][4 * i + 3]} * a;
-  __syncthreads();
-  f32x4 R[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    R[i] = f32x4{};
-#pragma unroll
-    for (int w = 0; w < kNarrowWaves; ++w) R[i] += *(lds_f32x4*)(x + w * 16384 + (wave * 4 + i) * 1024 + lane * 16);
-  }
-  if (!live) return;
-  if (j.state >= 0) {
-    float* st = p.part + (((long long)j.state * p.kv_heads + j.h) * p.row_tiles + (rho >> 5)) * kState;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<f32x4*>(st + ((8 * wave + 2 * i + hh) * 32 + (rho & 31)) * 4) = R[i];
-    if (wave == 0 && hh == 0) {
-      st[32 * kHeadDim + (rho & 31)] = M;
-      st[32 * kHeadDim + 32 + (rho & 31)] = L;
+  if constexpr (NW == 1) {
+    finish_row<F16, kNarrow>(p, j, O, mine, l, 0, e);
+  } else {
+    // the waves' states into one: every wave hands over m, l and its 32 x 128
+    // sums, [dim tile][j][lane] of 4 floats, two dim tiles at a time (8 KB a wave;
+    // all row loads have landed), and adds up its share
+    const int re = e & 31, he = e >> 5;
+    typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+    typedef __attribute__((address_space(3))) float lds_f32;
+    constexpr int kItems = 16 / NW;
+    lds_f32* const xm = (lds_f32*)(ring + NW * 8192);
+    __syncthreads();
+    if (he == 0) {
+      xm[wave * 64 + re] = mine;
+      xm[wave * 64 + 32 + re] = l;
     }
-    return;
-  }
-  const bool none = __float_as_uint(L) == 0u;
-  const float inv = none ? 0.0f : 1.0f / L;
-  uint16_t* op = p.out + (long long)token * p.o_tok + (long long)hq * p.o_head + 32 * wave + 4 * hh;
+    __syncthreads();
+    float M = -INFINITY, L = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    R[i] *= inv;
-    *reinterpret_cast<u32x2*>(op + 8 * i) = u32x2{pack2<F16>(R[i][0], R[i][1]), pack2<F16>(R[i][2], R[i][3])};
+    for (int w = 0; w < NW; ++w) M = __builtin_fmaxf(M, xm[w * 64 + re]);
+    const float Mu = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) L += xm[w * 64 + 32 + re] * __builtin_amdgcn_exp2f(xm[w * 64 + re] - Mu);
+    const float a = __builtin_amdgcn_exp2f(mine - Mu);
+    f32x4 R[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) R[i] = f32x4{};
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      if (part) __syncthreads();
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const f32x16& o = O[2 * part + (c >> 2)];
+        const int i = 4 * (c & 3);
+        *(lds_f32x4*)(ring + wave * 8192 + c * 1024 + e * 16) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]} * a;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int c = wave * kItems + i - 8 * part;
+        if (c >= 0 && c < 8) {
+#pragma unroll
+          for (int w = 0; w < NW; ++w) R[i] += *(lds_f32x4*)(ring + w * 8192 + c * 1024 + e * 16);
+        }
+      }
+    }
+    const int rho = j.rho0 + re;
+    if (rho >= j.rho1) return;
+    if (j.state >= 0) {
+      int col;
+      float* st = state_of<kNarrow>(p, j, rho, 0, &col);
+#pragma unroll
+      for (int i = 0; i < kItems; ++i)
+        *reinterpret_cast<f32x4*>(st + ((2 * (wave * kItems + i) + he) * 32 + col) * 4) = R[i];
+      if (wave == 0 && he == 0) {
+        st[32 * kHeadDim + col] = M;
+        st[32 * kHeadDim + 32 + col] = L;
+      }
+      return;
+    }
+    const int token = rho / p.group, hq = j.h * p.group + rho % p.group;
+    const bool none = __float_as_uint(L) == 0u;
+    const float inv = none ? 0.0f : 1.0f / L;
+    uint16_t* op = p.out + (long long)token * p.o_tok + (long long)hq * p.o_head + 4 * he;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      R[i] *= inv;
+      *reinterpret_cast<u32x2*>(op + 8 * (wave * kItems + i)) =
+          u32x2{pack2<F16>(R[i][0], R[i][1]), pack2<F16>(R[i][2], R[i][3])};
+    }
+    if (p.lse && wave == 0 && he == 0) p.lse[(long long)token * p.heads + hq] = lse_of(M, L);
   }
-  if (p.lse && wave == 0 && hh == 0)
-    p.lse[(long long)token * p.heads + hq] = none ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f;
 }
 
-// Joins the pieces' states of 32 rows of a K/V head, dims 32 dt ..: block (h,
-// tile, dt), wave w takes dims 8 w .. 8 w + 7.  Bound by the latency of its loads:
-// those of 8 pieces are out together.
+// APART: prefix tiles, then own tiles, a wave each.
+template <bool F16, bool APART>
+__global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParams p) {
+  __shared__ alignas(16) uint8_t ring[kNarrowWaves * 2 * kHalf];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int b = blockIdx.x, first = APART ? p.prefix_items : 0;
+  const int item = b < first ? xcd_remap(b, first) : xcd_remap(b - first, gridDim.x - first);
+  Job j;
+  if constexpr (APART) {
+    if (b < first) {
+      if (prefix_job<kNarrow>(p, item, j)) narrow_tile<F16, kNarrowWaves>(p, j, (lds_u8*)ring, lane, wave);
+    } else {
+      const int own = item * kNarrowWaves + wave;
+      if (own < p.kv_heads * p.own_tiles * p.own_pieces && own_job<kNarrow>(p, own, lane, j))
+        narrow_tile<F16, 1>(p, j, (lds_u8*)ring, lane, wave);
+    }
+  } else {
+    if (own_job<kNarrow>(p, item, lane, j)) narrow_tile<F16, kNarrowWaves>(p, j, (lds_u8*)ring, lane, wave);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Wide tiles: 256 rows.  Bound by the matrix pipe and the vector work of the
+// softmax together: eight waves, two on a SIMD, so that one's products run under
+// the other's exponentials; each holds 32 rows with their sums in registers and
+// walks every key, and all share the pages.  S^T = K Q^T and O^T += V^T P^T on
+// 32 x 32 x 16 products: a lane holds one query, its softmax needs no other lane
+// but l ^ 32.
+constexpr int kWide = 256, kWideWaves = 8, kSlots = 4;
+constexpr int kTile = 64 * 256;      // a page's K or V rows
+
+// Ring: kSlots pages of K, then of V.
+template <bool F16>
+__device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
+  const int r = lane & 31, hh = lane >> 5;
+  int limit;                                  // rows of its sequence that the lane's row sees
+  u32x4 qop[8];
+  {
+    const int rho = min(j.rho0 + 32 * wave + r, j.rho1 - 1);
+    const int token = rho / p.group, hq = j.h * p.group + rho % p.group;
+    limit = p.causal ? j.length - j.n + (token - j.first_token) + 1 : j.length;
+    const uint16_t* qp = p.q + (long long)token * p.q_tok + (long long)hq * p.q_head + 8 * hh;
+#pragma unroll
+    for (int st = 0; st < 8; ++st) qop[st] = ldg16(qp + 16 * st);
+  }
+  // what every row of the wave sees of its sequence; a wave without rows only
+  // loads
+  const int all_see = __builtin_amdgcn_readfirstlane(limit);
+  const bool alive = j.rho0 + 32 * wave < j.rho1;
+  const int units = j.prefix_pages + j.own_pages;
+  const int begin = (int)((long long)units * j.piece / j.pieces);
+  const int end = (int)((long long)units * (j.piece + 1) / j.pieces);
+
+  lds_u8* const kring = ring;
+  lds_u8* const vring = kring + kSlots * kTile;
+  // this wave loads rows 8 wave .. 8 wave + 7 of every page
+  uint32_t koff[4] = {}, voff[4] = {};
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj) {
+    const int row = 8 * wave + 4 * jj + (lane >> 4), c = lane & 15;
+    const uint32_t at = (uint32_t)(row * p.kv_tok);
+    koff[jj] = 2u * (at + 8u * (uint32_t)(c ^ (row & 15))) - 1024u * jj;
+    voff[jj] = 2u * (at + 8u * (uint32_t)(c ^ vswz(row))) - 1024u * jj;
+  }
+  const long long page_bytes = 128 * p.kv_tok;
+  const uint8_t* const kh = (const uint8_t*)(p.k + (long long)j.h * p.kv_head);
+  const uint8_t* const vh = (const uint8_t*)(p.v + (long long)j.h * p.kv_head);
+  PageList list(p, j, begin, lane);
+  int rows_ahead[kSlots] = {0, 0, 0, 0};    // rows of units i .. i + 3
+  auto issue = [&](int u) {
+    if (u >= end) return 0;
+    const Unit x = list.at(p, j, u, lane);
+    const long long at = max(x.page, 0) * page_bytes;
+    const uint32_t l =
+        __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)kring + ((u - begin) % kSlots) * kTile + wave * 2048);
+    dma_rows<2>(kh + at, koff, l);
+    dma_rows<2>(vh + at, voff, l + kSlots * kTile);
+    return x.rows;
+  };
+#pragma unroll
+  for (int u = 0; u < kSlots - 1; ++u) rows_ahead[u] = issue(begin + u);
+
+  f32x16 O[4], S;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
+  float m = -INFINITY, ls = 0.0f, nb, mx;
+  const uint32_t klane = (uint32_t)(r * 256 + ((hh ^ (r & 15)) << 4));
+  uint32_t vlane;
+  {
+    const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2);
+    vlane = (uint32_t)(row * 256 + (((2 * (g & 1) + ((i & 3) >> 1)) ^ vswz(row)) << 4) + (i & 1) * 8);
+  }
+  // rows of a page behind its end hold anything: 0 * NaN must not reach the
+  // sums, so each wave clears those of its V rows once they have landed
+  auto clear_rows = [&](int u, int rows) {
+    if (rows < kPage) {
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+        if (8 * wave + 4 * jj + (lane >> 4) >= rows)
+          *(lds_u32x4*)(vring + ((u - begin) % kSlots) * kTile + wave * 2048 + jj * 1024 + lane * 16) = u32x4{};
+    }
+  };
+  // whether some row does not see all keys of half page `half` of unit u, which
+  // holds `rows` rows; mask drops the scores of those it does not see
+  auto cut = [&](int u, int half, int rows) {
+    const int o = u - j.prefix_pages;
+    return (o >= 0 ? min(rows, all_see - kPage * o) : rows) < 32 * half + 32;
+  };
+  auto mask = [&](f32x16& X, int u, int half, int rows) {
+    const int o = u - j.prefix_pages;
+    int see = rows;
+    if (o >= 0) see = min(see, limit - kPage * o);
+    see -= 32 * half + 4 * hh;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) X[i] = 8 * (i / 4) + i % 4 < see ? X[i] : -INFINITY;
+  };
+  auto rescale = [&]() {
+    if (__any(mx > m + kSlack)) {
+      const float to = __builtin_fmaxf(m, mx);
+      const float a = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));
+      ls *= a;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
+      m = to;
+    }
+    nb = kLift<F16> - (m == -INFINITY ? 0.0f : m);
+  };
+  // Half a page: the probabilities of Sc meet V (rows 32 half .. of `vb`), with
+  // the scores Sn of the next half page (rows of `kb`) and their maximum.  ka
+  // holds the first four K operands on entry, and on return those of the half
+  // page after (rows of `kafter`).
+  u32x4 ka[8];
+  auto kread = [&](const lds_u8* kb, int x) { return *(lds_u32x4*)(kb + (klane ^ (uint32_t)(x << 5))); };
+  auto half_step = [&](const lds_u8* kb, const lds_u8* kafter, const lds_u8* vb, const f32x16& Sc, f32x16& Sn, int next,
+                       int next_half, int next_rows) {
+    u32x4 va[2][4], pb[2];
+    float P[16], ps = 0.0f;
+    auto vread = [&](int ks, int dt) {
+      const lds_u8* a = vb + 4096 * ks + (vlane ^ (uint32_t)(dt << 6));
+      return tr_pair(a, a + 2048);
+    };
+    auto expo = [&](int i) {
+      P[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(Sc[i], p.scale_log2, nb));
+      ps += P[i];
+      if (i & 1) pb[i >> 3][(i & 7) >> 1] = pack2<F16>(P[i - 1], P[i]);
+    };
+    auto group = []() { __builtin_amdgcn_sched_barrier(0); };
+    Sn = f32x16{};
+    group();
+#pragma unroll
+    for (int st = 0; st < 8; ++st) {
+      Sn = mma<F16>(ka[st], qop[st], Sn);
+      if (st < 4)
+        ka[st + 4] = kread(kb, st + 4);
+      else
+        va[0][st - 4] = vread(0, st - 4);
+      expo(st);
+      if (st & 1) expo(8 + st / 2);
+      group();
+    }
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) {
+      O[dt] = mma<F16>(va[0][dt], pb[0], O[dt]);
+      va[1][dt] = vread(1, dt);
+      expo(12 + dt);
+      group();
+    }
+    float part;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) {
+      O[dt] = mma<F16>(va[1][dt], pb[1], O[dt]);
+      ka[dt] = kread(kafter, dt);
+      if (dt == 0) part = lane_max(Sn);
+      if (dt == 1) mx = half_max(part) * p.scale_log2;
+      if (dt == 2) {
+        ls += ps;
+        asm volatile("" : "+v"(ls));   // here, not behind the branches below
+      }
+      group();
+    }
+    if (cut(next, next_half, next_rows)) {
+      mask(Sn, next, next_half, next_rows);
+      mx = half_max(lane_max(Sn)) * p.scale_log2;
+    }
+    rescale();
+  };
+
+  if (begin < end) {
+    wait_loads();
+    clear_rows(begin, rows_ahead[0]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    S = f32x16{};
+    if (alive) {
+#pragma unroll
+      for (int st = 0; st < 8; ++st) S = mma<F16>(kread(kring, st), qop[st], S);
+    }
+    if (cut(begin, 0, rows_ahead[0])) mask(S, begin, 0, rows_ahead[0]);
+    mx = half_max(lane_max(S)) * p.scale_log2;
+    rescale();
+#pragma unroll
+    for (int st = 0; st < 4; ++st) ka[st] = kread(kring + kTile / 2, st);
+    for (int u = begin; u < end; ++u) {
+      rows_ahead[3] = issue(u + 3);
+      const int slot = (u - begin) % kSlots, after = (u + 1 - begin) % kSlots;
+      const lds_u8 *k0 = kring + slot * kTile, *k1 = kring + after * kTile, *v = vring + slot * kTile;
+      f32x16 S1;
+      if (alive) {
+        half_step(k0 + kTile / 2, k1, v, S, S1, u, 1, rows_ahead[0]);
+        half_step(k1, k1 + kTile / 2, v + kTile / 2, S1, S, u + 1, 0, rows_ahead[1]);
+      }
+      // next: K of unit u + 2 and V of unit u + 1; each unit is 2 loads of K,
+      // then 2 of V
+      if (u + 3 < end)
+        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      rows_ahead[0] = rows_ahead[1];
+      rows_ahead[1] = rows_ahead[2];
+      rows_ahead[2] = rows_ahead[3];
+      if (u + 1 < end) clear_rows(u + 1, rows_ahead[0]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+    }
+  }
+
+  // the lane's row, formed anew so that no register holds it across the loop
+  int e = lane;
+  asm volatile("" : "+v"(e));
+  finish_row<F16, kWide>(p, j, O, m == -INFINITY ? m : m - kLift<F16>, half_sum(ls), wave, e);
+}
+
+// APART: prefix tiles, then own tiles of 32 rows, eight to a workgroup, a wave
+// each.
+template <bool F16, bool APART>
+__global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p) {
+  __shared__ alignas(16) uint8_t ring[2 * kSlots * kTile];
+  static_assert(sizeof(ring) >= kWideWaves * 2 * kHalf);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int b = blockIdx.x, first = APART ? p.prefix_items : p.own_whole;
+  // the longer items first; either kind by itself over the XCDs
+  const int item = b < first ? xcd_remap(b, first) : xcd_remap(b - first, gridDim.x - first);
+  Job j;
+  if constexpr (APART) {
+    if (b < first) {
+      if (prefix_job<kWide>(p, item, j)) wide_tile<F16>(p, j, (lds_u8*)ring, lane, wave);
+    } else {
+      const int own = item * kWideWaves + wave;
+      if (own < p.kv_heads * p.own_tiles * p.own_pieces && own_job<kNarrow>(p, own, lane, j))
+        narrow_tile<F16, 1>(p, j, (lds_u8*)ring, lane, wave);
+    }
+  } else {
+    if (own_job<kWide>(p, b < first ? item : first + item, lane, j))
+      wide_tile<F16>(p, j, (lds_u8*)ring, lane, wave);
+  }
+}
+
+// Joins the pieces' states of 32 rows of a K/V head, dims 32 dt ..: block (h, rows
+// 32 T .., dt) where the prefix is apart (T_ROWS 0), else (split tile of T_ROWS
+// rows, block of 32, dt); wave w takes dims 8 w .. 8 w + 7.  Bound by the latency
+// of its loads: those of 8 pieces are out together.
 constexpr int kJoin = 8;
 
-template <bool F16>
-__global__ __launch_bounds__(256) void join_kernel(PagedParams p, int pieces) {
+template <bool F16, int T_ROWS>
+__global__ __launch_bounds__(256) void join_kernel(PagedParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int dt = blockIdx.x & 3, T = (blockIdx.x >> 2) % p.row_tiles, h = (blockIdx.x >> 2) / p.row_tiles;
-  const int r = lane & 31, hh = lane >> 5;
-  const int rho = 32 * T + r;
-  const bool live = rho < packed_tokens(p) * p.group;
-  const long long step = (long long)p.kv_heads * p.row_tiles * kState;
-  const float* st = p.part + ((long long)h * p.row_tiles + T) * kState;
+  const int dt = blockIdx.x & 3, block = blockIdx.x >> 2, r = lane & 31, hh = lane >> 5;
+  int h, rho, end, pieces;
+  long long step;                 // floats from a piece to the next
+  const float* st;
+  if constexpr (T_ROWS == 0) {
+    h = block / p.row_tiles;
+    rho = 32 * (block - h * p.row_tiles) + r;
+    end = packed_tokens(p) * p.group;
+    pieces = p.prefix_pieces + p.own_pieces;
+    step = (long long)p.kv_heads * p.row_tiles * kState;
+    st = p.part + (long long)block * kState;
+  } else {
+    constexpr int kBlocks = T_ROWS / 32;
+    const int t = block / kBlocks, blk = block - t * kBlocks;
+    Job j;
+    if (!find_rows<T_ROWS>(p, p.own_whole + t, lane, j)) return;
+    h = j.h;
+    rho = j.rho0 + 32 * blk + r;
+    end = j.rho1;
+    pieces = p.own_pieces;
+    step = (long long)kBlocks * kState;
+    st = p.part + ((long long)t * pieces * kBlocks + blk) * kState;
+  }
+  const bool live = rho < end;
   float M = -INFINITY, L = 0.0f;
   f32x4 acc = {};
   for (int c = 0; c < pieces; c += kJoin, st += kJoin * step) {
@@ -517,17 +888,40 @@ __global__ __launch_bounds__(256) void join_kernel(PagedParams p, int pieces) {
   *reinterpret_cast<u32x2*>(p.out + (long long)token * p.o_tok + (long long)hq * p.o_head + 32 * dt + 8 * wave + 4 * hh) =
       u32x2{pack2<F16>(acc[0], acc[1]), pack2<F16>(acc[2], acc[3])};
   if (p.lse && dt == 0 && wave == 0 && hh == 0)
-    p.lse[(long long)token * p.heads + hq] = none ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f;
+    p.lse[(long long)token * p.heads + hq] = lse_of(M, L);
 }
 
-// How a call is cut up, from sizes alone.
+// How a call is cut up, from sizes alone.  Tiles are of 32 rows (narrow) or 256
+// (wide); own tiles beside prefix tiles are narrow.
 struct Plan {
-  int row_tiles, prefix_tiles, prefix_pieces, own_tiles, own_pieces;
-  bool split() const { return prefix_tiles > 0 || own_pieces > 1; }
-  long long bytes(int kv_heads) const {
-    return split() ? 4ll * kState * (prefix_pieces + own_pieces) * kv_heads * row_tiles : 0;
+  int rows, row_tiles, prefix_tiles, prefix_pieces, own_tiles, own_whole, own_pieces;
+  bool apart() const { return prefix_tiles > 0; }
+  long long split_tiles(int kv_heads) const { return (long long)kv_heads * own_tiles - own_whole; }
+  long long states(int kv_heads) const {
+    if (apart()) return (long long)(prefix_pieces + own_pieces) * kv_heads * row_tiles;
+    return own_pieces > 1 ? split_tiles(kv_heads) * own_pieces * (rows / 32) : 0;
   }
+  long long bytes(int kv_heads) const { return 4ll * kState * states(kv_heads); }
 };
+
+// Estimates, in us, that the pieces are chosen by: a workgroup's start and end,
+// a page of a tile, a state written and read again.
+constexpr double kStart = 7.0, kJoinStart = 3.0, kSoloPage = 5.0, kNarrowPage = 0.75;
+double wide_page(double rows) { return 1.0 + 0.9 * std::min(1.0, rows / kWide); }
+double state_time(double rows) { return rows * 2 * (4.0 * kState / 32) / 4.5e6; }
+double page_time(double pages) { return pages * 32768 / 5.2e6; }
+
+constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64};
+
+// When n workgroups of the time t each, and then m of the time u, are done on
+// `slots` places.
+double makespan(double n, double t, double m, double u, double slots) {
+  const double rounds = std::ceil(n / slots), done = rounds * t;
+  const double left = rounds * slots - n;                     // places that the last round leaves
+  const double after = done + std::ceil(std::max(0.0, m - left * std::floor(t / u)) / slots) * u;
+  const double beside = left > 0 ? done - t + std::ceil(m / left) * u : after;
+  return std::max(done, std::min(after, beside));
+}
 
 bool sizes_fit(int tokens, int batch, int heads, int kv_heads, int prefix_tokens, int table_pages, bool ragged) {
   return tokens > 0 && batch > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && prefix_tokens >= 0 &&
@@ -535,26 +929,105 @@ bool sizes_fit(int tokens, int batch, int heads, int kv_heads, int prefix_tokens
          (long long)table_pages * kPage < (1ll << 30) && prefix_tokens < (1 << 30) && batch <= (1 << 20);
 }
 
+// Tiles over all heads of T rows, of sequences by themselves.
+int seq_tiles(long long rows, int batch, bool ragged, int T) {
+  return (int)(ragged ? rows / T + batch : (long long)batch * ((rows / batch + T - 1) / T));
+}
+
+// The prefix apart: all rows together over the prefix, each sequence over its own
+// pages.  Returns the estimated time.
+double plan_apart(int cus, long long rows, int batch, int kv_heads, int prefix_pages, int table_pages, bool ragged,
+                  Plan* plan) {
+  const int T = rows <= kNarrow ? kNarrow : kWide;
+  const bool wide = T == kWide;
+  const int slots = wide ? cus : 2 * cus, waves = wide ? kWideWaves : kNarrowWaves;
+  plan->rows = T;
+  plan->row_tiles = (int)((rows + 31) / 32);
+  plan->prefix_tiles = (int)((rows + T - 1) / T);
+  plan->own_tiles = seq_tiles(rows, batch, ragged, kNarrow);
+  plan->own_whole = 0;
+  const double tiles = (double)kv_heads * plan->prefix_tiles, own_tiles = (double)kv_heads * plan->own_tiles;
+  const double page = wide ? wide_page((double)rows / plan->prefix_tiles) : kNarrowPage;
+  const double floor_time = page_time(kv_heads * (prefix_pages + 0.6 * batch * table_pages));
+  double least = 1e30;
+  for (int c : kCuts) {
+    if (c > 1 && 2 * c > prefix_pages) break;
+    const double t = kStart + (prefix_pages + c - 1) / c * page;
+    for (int d : kCuts) {
+      if (d > 16 || (d > 1 && 2 * d > table_pages)) break;
+      const double u = kStart + (table_pages + d - 1) / d * kSoloPage;
+      const double cost = std::max(floor_time, makespan(tiles * c, t, own_tiles * d / waves, u, slots)) +
+                          state_time((double)kv_heads * rows * (c + d)) + kJoinStart;
+      if (cost < least) {
+        least = cost;
+        plan->prefix_pieces = c;
+        plan->own_pieces = d;
+      }
+    }
+  }
+  return least;
+}
+
+// Every tile over prefix and own pages.  With more wide tiles than CUs, only
+// those behind the last full round are cut.
+double plan_joint(int cus, long long rows, int batch, int kv_heads, int prefix_pages, int table_pages, bool ragged,
+                  Plan* plan) {
+  const double per_seq = (double)rows / batch;
+  const int T = per_seq <= kNarrow ? kNarrow : kWide;
+  const bool wide = T == kWide;
+  const int slots = wide ? cus : 2 * cus;
+  plan->rows = T;
+  plan->row_tiles = plan->prefix_tiles = plan->prefix_pieces = 0;
+  plan->own_tiles = seq_tiles(rows, batch, ragged, T);
+  const long long own_tiles = (long long)kv_heads * plan->own_tiles, whole = wide ? own_tiles / cus * cus : 0;
+  const int units = table_pages + prefix_pages;
+  const double tiles = (double)(own_tiles - whole);
+  const double live = per_seq / std::ceil(per_seq / T);     // rows of a tile that there are
+  const double page = wide ? wide_page(live) : kNarrowPage;
+  double least = tiles > 0 ? 1e30 : 0.0;
+  plan->own_pieces = 1;
+  for (int c : kCuts) {
+    if (tiles == 0 || (c > 1 && 2 * c > units)) break;
+    const int pages = (units + c - 1) / c;
+    const double rounds = std::ceil(tiles * c / slots);
+    const double cost = rounds * std::max(kStart + pages * page, page_time(std::min(tiles * c, (double)slots) * pages)) +
+                        (c > 1 ? state_time(tiles * c * live) + kJoinStart : 0.0);
+    if (cost < least) {
+      least = cost;
+      plan->own_pieces = c;
+    }
+  }
+  plan->own_whole = (int)(plan->own_pieces == 1 ? own_tiles : whole);
+  return least + (double)(whole / cus) * (kStart + units * page);
+}
+
+// The plan of a call's sizes.  A thread keeps its last one: the estimates of all
+// cuts take longer than a launch.
 int make_plan(int tokens, int batch, int heads, int kv_heads, int prefix_tokens, int table_pages, bool ragged,
               Plan* plan) {
   int cus = 0;
   const int e = device_cus(&cus);
   if (e != (int)hipSuccess) return e;
-  const int group = heads / kv_heads;
-  const long long rows = (long long)tokens * group;
-  const int prefix_pages = (prefix_tokens + kPage - 1) / kPage;
-  plan->row_tiles = (int)((rows + 31) / 32);
-  const long long own_tiles =
-      ragged ? rows / kNarrow + batch : (long long)batch * ((rows / batch + kNarrow - 1) / kNarrow);
-  plan->own_tiles = (int)own_tiles;
-  const bool together = batch > 1 && prefix_pages > 0 && rows < 32ll * batch;
-  auto pieces = [&](long long tiles, int units) {
-    const long long fill = std::max(1ll, cus / std::max(1ll, tiles));
-    return (int)std::min(fill, (long long)std::max(1, units / 4));
+  struct Last {
+    std::array<int, 8> sizes{};
+    Plan plan;
   };
-  plan->prefix_tiles = together ? plan->row_tiles : 0;
-  plan->prefix_pieces = together ? pieces((long long)kv_heads * plan->prefix_tiles, prefix_pages) : 0;
-  plan->own_pieces = pieces(kv_heads * own_tiles, table_pages + (together ? 0 : prefix_pages));
+  static thread_local Last last;
+  const std::array<int, 8> sizes = {cus, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, (int)ragged};
+  if (sizes == last.sizes) {
+    *plan = last.plan;
+    return (int)hipSuccess;
+  }
+  const long long rows = (long long)tokens * (heads / kv_heads);
+  const int prefix_pages = (prefix_tokens + kPage - 1) / kPage;
+  const double joint = plan_joint(cus, rows, batch, kv_heads, prefix_pages, table_pages, ragged, plan);
+  if (batch > 1 && prefix_pages > 0) {
+    Plan other;
+    const double apart = plan_apart(cus, rows, batch, kv_heads, prefix_pages, table_pages, ragged, &other);
+    if (apart < joint) *plan = other;
+  }
+  last.sizes = sizes;
+  last.plan = *plan;
   return (int)hipSuccess;
 }
 
@@ -626,22 +1099,42 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   p.prefix_tiles = plan.prefix_tiles;
   p.prefix_pieces = plan.prefix_pieces;
   p.own_tiles = plan.own_tiles;
+  p.own_whole = plan.own_whole;
   p.own_pieces = plan.own_pieces;
-  const long long items = (long long)kv_heads * (1ll * plan.prefix_tiles * plan.prefix_pieces +
-                                                 1ll * plan.own_tiles * plan.own_pieces);
-  if (items > 0x7fffffffll || 4ll * kv_heads * plan.row_tiles > 0x7fffffffll) return (int)hipErrorInvalidValue;
+  p.apart = plan.apart();
+  const long long prefix_items = 1ll * kv_heads * plan.prefix_tiles * plan.prefix_pieces;
+  const bool wide = plan.rows == kWide;
+  long long own_items = plan.own_whole + plan.split_tiles(kv_heads) * plan.own_pieces;
+  if (own_items > 0x7fffffffll) return (int)hipErrorInvalidValue;
+  const int waves = wide ? kWideWaves : kNarrowWaves;
+  if (plan.apart()) own_items = (own_items + waves - 1) / waves;    // a wave each
+  const long long items = prefix_items + own_items;
+  const long long joins = plan.apart() ? 4ll * kv_heads * plan.row_tiles
+                                       : plan.own_pieces > 1 ? plan.split_tiles(kv_heads) * (plan.rows / 8) : 0;
+  if (items > 0x7fffffffll || joins > 0x7fffffffll) return (int)hipErrorInvalidValue;
+  p.prefix_items = (int)prefix_items;
   const bool f16 = flags & 1;
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)items), dim3(64 * kNarrowWaves), 0, stream, p);
+  auto launch = [&](auto kernel, long long blocks, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, p);
   };
-  f16 ? launch(narrow_kernel<true>) : launch(narrow_kernel<false>);
-  if (plan.split()) {
-    const dim3 grid(4 * kv_heads * plan.row_tiles);
-    const int pieces = plan.prefix_pieces + plan.own_pieces;
-    if (f16)
-      hipLaunchKernelGGL(join_kernel<true>, grid, dim3(256), 0, stream, p, pieces);
+  auto start = [&](auto f16_apart, auto bf16_apart, auto f16_joint, auto bf16_joint) {
+    if (plan.apart())
+      f16 ? launch(f16_apart, items, 64 * waves) : launch(bf16_apart, items, 64 * waves);
     else
-      hipLaunchKernelGGL(join_kernel<false>, grid, dim3(256), 0, stream, p, pieces);
+      f16 ? launch(f16_joint, items, 64 * waves) : launch(bf16_joint, items, 64 * waves);
+  };
+  if (wide)
+    start(wide_kernel<true, true>, wide_kernel<false, true>, wide_kernel<true, false>, wide_kernel<false, false>);
+  else
+    start(narrow_kernel<true, true>, narrow_kernel<false, true>, narrow_kernel<true, false>,
+          narrow_kernel<false, false>);
+  if (joins > 0) {
+    if (plan.apart())
+      f16 ? launch(join_kernel<true, 0>, joins, 256) : launch(join_kernel<false, 0>, joins, 256);
+    else if (!wide)
+      f16 ? launch(join_kernel<true, kNarrow>, joins, 256) : launch(join_kernel<false, kNarrow>, joins, 256);
+    else
+      f16 ? launch(join_kernel<true, kWide>, joins, 256) : launch(join_kernel<false, kWide>, joins, 256);
   }
   return (int)hipGetLastError();
 }

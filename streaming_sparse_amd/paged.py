@@ -20,65 +20,96 @@ import math
 import torch
 
 from . import _lib
-from .legacy_components import HEAD_DIM, kv_strides
+from .legacy_components import HEAD_DIM
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _INT, _F64 = torch.int32, torch.float64
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, '_cuda_getDevice') else torch.cuda.current_device
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
-def _cache(cache_k, cache_v, dtype, device):
-    """(pages, K/V heads, token stride, head stride) of the resident cache."""
-    shape = cache_k.shape
-    if len(shape) != 4 or shape[0] != 1 or shape[3] != HEAD_DIM or shape[1] == 0 or shape[1] % 64 or \
-            cache_v.shape != shape:
-        raise ValueError("cache_k and cache_v must be [1, 64P, G, 128] of equal shape")
+# The checks below stand in the path of a call of a few microseconds, so each
+# property of a tensor is asked for once and devices are compared by index.
+
+def _overlap(rows, heads, tok, head):
+    """Whether rows of 128 elements at r * tok + h * head may share elements:
+    neither do the heads of a token lie between two tokens, nor the tokens of
+    a head between two heads."""
+    return (tok < (heads - 1) * head + HEAD_DIM and rows > 1 or head < HEAD_DIM and heads > 1) and \
+        (head < (rows - 1) * tok + HEAD_DIM and heads > 1 or tok < HEAD_DIM and rows > 1)
+
+
+def _cache(cache_k, cache_v, dtype, dev):
+    """(rows, K/V heads, token stride, head stride) of the resident cache."""
+    shape, stride = cache_k.shape, cache_k.stride()
     if cache_k.dtype is not dtype or cache_v.dtype is not dtype:
         raise TypeError("the cache must have the new rows' dtype (bfloat16 or float16)")
-    if cache_k.device != device or cache_v.device != device:
+    if len(shape) != 4 or cache_v.shape != shape or cache_v.stride() != stride:
+        raise ValueError("cache_k and cache_v must be [1, 64P, G, 128] of equal shape and strides")
+    one, rows, heads, dim = shape
+    _, tok, head, unit = stride
+    if one != 1 or dim != HEAD_DIM or rows == 0 or rows & 63 or heads == 0:
+        raise ValueError("cache_k and cache_v must be [1, 64P, G, 128]")
+    if unit != 1 or (tok | head) & 7 or (cache_k.data_ptr() | cache_v.data_ptr()) & 15 or tok < HEAD_DIM or \
+            _overlap(rows, heads, tok, head):
+        raise ValueError("the cache's rows must not overlap and must start at multiples of 16 bytes")
+    if cache_k.get_device() != dev or cache_v.get_device() != dev:
         raise ValueError("the cache must be on the new rows' device")
-    tok, head = kv_strides(cache_k, cache_v)
-    return shape[1] // 64, shape[2], tok, head
+    return rows, heads, tok, head
 
 
-def _rows(x, name, dtype, device):
-    """(token stride, head stride) of packed rows [N, heads, 128]."""
-    shape, stride = x.shape, x.stride()
+def _rows(x, name, dtype, dev):
+    """(N, heads, token stride, head stride, pointer) of packed rows [N, heads, 128]."""
+    shape, stride, ptr = x.shape, x.stride(), x.data_ptr()
     if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1:
         raise ValueError(f"{name} must be [N, heads, 128] with adjacent elements in a row")
-    if x.dtype is not dtype or x.device != device:
+    tokens, heads, _ = shape
+    tok, head, _ = stride
+    if x.dtype is not dtype or x.get_device() != dev:
         raise TypeError(f"{name} must share the other rows' dtype and device")
-    if (stride[0] | stride[1]) & 7 or x.data_ptr() & 15:
+    if (tok | head) & 7 or ptr & 15:
         raise ValueError(f"{name}'s rows must start at multiples of 16 bytes")
-    return stride[0], stride[1]
+    return tokens, heads, tok, head, ptr
 
 
-def _ints(x, name, shape, device):
-    if x.dtype is not _INT or x.shape != shape or not x.is_contiguous() or x.device != device:
+def _written(x, name, dtype, dev):
+    """_rows of a tensor that is written: its rows must not overlap."""
+    got = _rows(x, name, dtype, dev)
+    if _overlap(*got[:4]):
+        raise ValueError(f"{name}'s rows must not overlap")
+    return got
+
+
+def _ints(x, name, shape, dev):
+    if x.dtype is not _INT or x.shape != shape or not x.is_contiguous() or x.get_device() != dev:
         raise ValueError(f"{name} must be a contiguous int32 {list(shape)} tensor on the rows' device")
     return x.data_ptr()
 
 
-def _sequences(table, starts, tokens, device):
-    """(batch, pages a sequence may own, starts pointer)."""
-    if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
+def _sequences(table, starts, tokens, dev):
+    """(batch, pages a sequence may own, table pointer, starts pointer)."""
+    if table.dim() != 2:
         raise ValueError("table must be [B, M]")
-    batch, width = table.shape
+    batch, width = shape = table.shape
+    if batch == 0 or width == 0:
+        raise ValueError("table must be [B, M]")
+    ptr = _ints(table, "table", shape, dev)
     if starts is None:
         if tokens % batch:
             raise ValueError("without starts, the sequences have N / B new tokens each: N must be a multiple of B")
-        return batch, width, None
-    return batch, width, _ints(starts, "starts", (batch + 1,), device)
+        return batch, width, ptr, None
+    return batch, width, ptr, _ints(starts, "starts", (batch + 1,), dev)
 
 
-def _on(device, call):
-    """call() with `device` current."""
-    if device.type != 'cuda':
+def _launch(name, device, dev, *args):
+    """The library's entry `name` with `device` current, on its current stream."""
+    if dev < 0:
         raise RuntimeError("the tensors must be on a GPU")
-    if device.index is None or device.index == _current_device():
-        return call()
-    with torch.cuda.device(device):
-        return call()
+    fn = getattr(_lib.lib(), name)
+    if dev == torch.cuda.current_device():
+        _lib.check(fn(*args, _lib.stream_handle(device)), name)
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, _lib.stream_handle(device)), name)
 
 
 def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=None, freqs=None, axes=None,
@@ -103,62 +134,61 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
     q_out: where the rotated queries go (q itself is allowed); else a buffer
     owned by `workspace` that the next call overwrites, or, without one, a new
     tensor."""
-    device, dtype = k.device, k.dtype
+    device, dtype, dev = k.device, k.dtype, k.get_device()
     code = _TYPES.get(dtype)
     if code is None:
         raise TypeError("k must be bfloat16 or float16")
-    k_tok, k_head = _rows(k, "k", dtype, device)
-    v_tok, v_head = _rows(v, "v", dtype, device)
-    n, g, _ = k.shape
-    pages, gc, kv_tok, kv_head = _cache(cache_k, cache_v, dtype, device)
-    if v.shape != k.shape or gc != g:
+    n, g, k_tok, k_head, k_ptr = _rows(k, "k", dtype, dev)
+    nv, gv, v_tok, v_head, v_ptr = _rows(v, "v", dtype, dev)
+    rows, gc, kv_tok, kv_head = _cache(cache_k, cache_v, dtype, dev)
+    if nv != n or gv != g or gc != g:
         raise ValueError("k and v must be [N, G, 128] for the cache's G heads")
-    batch, width, starts_ptr = _sequences(table, starts, n, device)
-    table_ptr, held_ptr = _ints(table, "table", (batch, width), device), _ints(held, "held", (batch,), device)
+    batch, width, table_ptr, starts_ptr = _sequences(table, starts, n, dev)
+    held_ptr = _ints(held, "held", (batch,), dev)
     pairs, a0, a1, na, freqs_ptr, pos_ptr = 0, 0, 0, 1, None, None
     if freqs is not None:
-        if freqs.dtype is not _F64 or freqs.dim() != 1 or freqs.device != device or not freqs.is_contiguous():
+        if freqs.dtype is not _F64 or freqs.dim() != 1 or freqs.get_device() != dev or not freqs.is_contiguous():
             raise ValueError("freqs must be a contiguous float64 [R] tensor on the rows' device")
         pairs, freqs_ptr = freqs.shape[0], freqs.data_ptr()
         if pairs > HEAD_DIM // 2 or (not interleaved and pairs % 8):
             raise ValueError("at most 64 pairs, a multiple of 8 in halves")
-        counts = (pairs,) if axes is None else tuple(axes)
-        na = len(counts)
-        if not 1 <= na <= 3 or sum(counts) != pairs or min(counts) < 0:
-            raise ValueError("axes must be 1 to 3 counts that sum to the pairs")
-        a0, a1 = counts[0], counts[1] if na > 1 else 0
+        if axes is None:
+            a0 = pairs
+        else:
+            na = len(axes)
+            if not 1 <= na <= 3 or sum(axes) != pairs or min(axes) < 0:
+                raise ValueError("axes must be 1 to 3 counts that sum to the pairs")
+            a0, a1 = axes[0], axes[1] if na > 1 else 0
         if positions is not None:
-            pos_ptr = _ints(positions, "positions", (n,) if positions.dim() == 1 and na == 1 else (n, na), device)
+            pos_ptr = _ints(positions, "positions", (n,) if na == 1 and positions.dim() == 1 else (n, na), dev)
         elif na > 1:
             raise ValueError("several axes need positions")
     elif positions is not None or axes is not None:
         raise ValueError("positions and axes need freqs")
     h, q_ptr, out_ptr, q_tok, q_head, o_tok, o_head = 0, None, None, 0, 0, 0, 0
     if q is not None:
-        q_tok, q_head = _rows(q, "q", dtype, device)
-        h = q.shape[1]
-        if q.shape[0] != n or h == 0:
+        nq, h, q_tok, q_head, q_ptr = _rows(q, "q", dtype, dev)
+        if nq != n or h == 0:
             raise ValueError("q must be [N, H, 128]")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=dtype, device=device) if workspace is None else \
-                workspace.tensor('paged_q', q.shape, device, dtype)
-        elif q_out.shape != q.shape:
-            raise ValueError("q_out must have q's shape")
-        o_tok, o_head = _rows(q_out, "q_out", dtype, device)
-        q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
+            q_out = torch.empty((n, h, HEAD_DIM), dtype=dtype, device=device) if workspace is None else \
+                workspace.tensor('paged_q', (n, h, HEAD_DIM), device, dtype)
+            o_tok, o_head, out_ptr = h * HEAD_DIM, HEAD_DIM, q_out.data_ptr()
+        else:
+            no, ho, o_tok, o_head, out_ptr = _written(q_out, "q_out", dtype, dev)
+            if no != n or ho != h:
+                raise ValueError("q_out must have q's shape")
     elif q_out is not None:
         raise ValueError("q_out without q")
-    if n == 0:
-        return q_out
-    _on(device, lambda: _lib.check(_lib.lib().ssa_paged_append(
-        q_ptr, q_tok, q_head, out_ptr, o_tok, o_head, k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok, v_head,
-        cache_k.data_ptr(), cache_v.data_ptr(), kv_tok, kv_head, table_ptr, held_ptr, starts_ptr, pos_ptr, freqs_ptr,
-        first, n, batch, h, g, pages, width, pairs, a0, a1, na, code | (2 if interleaved else 0),
-        _lib.stream_handle(device)), "ssa_paged_append"))
+    if n:
+        _launch("ssa_paged_append", device, dev, q_ptr, q_tok, q_head, out_ptr, o_tok, o_head, k_ptr, k_tok, k_head,
+                v_ptr, v_tok, v_head, cache_k.data_ptr(), cache_v.data_ptr(), kv_tok, kv_head, table_ptr, held_ptr,
+                starts_ptr, pos_ptr, freqs_ptr, first, n, batch, h, g, rows >> 6, width, pairs, a0, a1, na,
+                code | 2 if interleaved else code)
     return q_out
 
 
-_BYTES = {}
+_BYTES = {}     # workspace bytes by sizes and device
 
 
 def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, workspace, *, starts=None, causal=True,
@@ -187,55 +217,60 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     probability meets V in 16 bits: in two parts (hi + lo) where a tile is
     bound by memory, in one where by the matrix pipe (fp16: scaled up by
     2^7)."""
-    device, dtype = q.device, q.dtype
+    device, dtype, dev = q.device, q.dtype, q.get_device()
     code = _TYPES.get(dtype)
     if code is None:
         raise TypeError("q must be bfloat16 or float16")
-    q_tok, q_head = _rows(q, "q", dtype, device)
-    n, h, _ = q.shape
-    pages, g, kv_tok, kv_head = _cache(cache_k, cache_v, dtype, device)
+    n, h, q_tok, q_head, q_ptr = _rows(q, "q", dtype, dev)
+    rows, g, kv_tok, kv_head = _cache(cache_k, cache_v, dtype, dev)
     if h == 0 or h % g:
         raise ValueError("the query heads must be a multiple of the cache's heads")
-    batch, width, starts_ptr = _sequences(table, starts, n, device)
-    table_ptr, len_ptr = _ints(table, "table", (batch, width), device), _ints(lengths, "lengths", (batch,), device)
+    batch, width, table_ptr, starts_ptr = _sequences(table, starts, n, dev)
+    len_ptr = _ints(lengths, "lengths", (batch,), dev)
     prefix_ptr = None
-    if prefix_tokens < 0:
-        raise ValueError("prefix_tokens must not be negative")
     if prefix_tokens > 0:
-        if prefix is None or prefix.dim() != 1 or 64 * prefix.shape[0] < prefix_tokens:
+        if prefix is None or prefix.dim() != 1 or prefix.shape[0] << 6 < prefix_tokens:
             raise ValueError("prefix must list the pages of prefix_tokens rows")
-        prefix_ptr = _ints(prefix, "prefix", prefix.shape, device)
-    scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
+        prefix_ptr = _ints(prefix, "prefix", prefix.shape, dev)
+    elif prefix_tokens < 0:
+        raise ValueError("prefix_tokens must not be negative")
+    if scale is None:
+        scale = _SCALE
+    elif not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive")
     if out is None:
-        out = workspace.tensor('paged_out', q.shape, device, dtype)
-    elif out.shape != q.shape:
-        raise ValueError("out must have q's shape")
-    o_tok, o_head = _rows(out, "out", dtype, device)
+        out = workspace.tensor('paged_out', (n, h, HEAD_DIM), device, dtype)
+        o_tok, o_head, out_ptr = h * HEAD_DIM, HEAD_DIM, out.data_ptr()
+    else:
+        no, ho, o_tok, o_head, out_ptr = _written(out, "out", dtype, dev)
+        if no != n or ho != h:
+            raise ValueError("out must have q's shape")
     lse = workspace.tensor('paged_lse', (n, h), device, torch.float32) if want_lse else None
     if n:
-        _on(device, lambda: _attend(
-            q.data_ptr(), q_tok, q_head, cache_k.data_ptr(), cache_v.data_ptr(), kv_tok, kv_head, prefix_ptr,
-            prefix_tokens, table_ptr, len_ptr, starts_ptr, out.data_ptr(), o_tok, o_head,
-            None if lse is None else lse.data_ptr(), n, batch, h, g, pages, width, scale,
-            code | (2 if causal else 0), workspace, device))
+        key = (n, batch, h, g, prefix_tokens, width, starts is None, dev)
+        need = _BYTES.get(key)
+        if need is None:
+            need = _workspace_bytes(key, device)
+        part = workspace.tensor('paged_part', (need,), device, torch.uint8).data_ptr() if need else None
+        _launch("ssa_paged_attention", device, dev, q_ptr, q_tok, q_head, cache_k.data_ptr(), cache_v.data_ptr(),
+                kv_tok, kv_head, prefix_ptr, prefix_tokens, table_ptr, len_ptr, starts_ptr, out_ptr, o_tok, o_head,
+                None if lse is None else lse.data_ptr(), n, batch, h, g, rows >> 6, width, scale,
+                code | 2 if causal else code, part, need)
     return (out, lse) if want_lse else out
 
 
-def _attend(*args):
-    *call, workspace, device = args
-    starts, prefix_tokens = call[11], call[8]
-    tokens, batch, heads, kv_heads, _, width = call[16:22]
-    key = (tokens, batch, heads, kv_heads, prefix_tokens, width, starts is not None, device)
-    need = _BYTES.get(key)
-    if need is None:
+def _workspace_bytes(key, device):
+    """The workspace that a call of these sizes needs, asked of the library once
+    per sizes and device."""
+    tokens, batch, heads, kv_heads, prefix_tokens, width, equal, dev = key
+    if dev < 0:
+        raise RuntimeError("the tensors must be on a GPU")
+    with torch.cuda.device(device):
         need = _lib.lib().ssa_paged_attention_workspace_bytes(tokens, batch, heads, kv_heads, prefix_tokens, width,
-                                                              int(starts is not None))
-        if need < 0:
-            raise ValueError("paged.attention: sizes out of range")
-        if len(_BYTES) > 4096:
-            _BYTES.clear()
-        _BYTES[key] = need
-    part = workspace.tensor('paged_part', (need,), device, torch.uint8).data_ptr() if need else None
-    _lib.check(_lib.lib().ssa_paged_attention(*call, part, need, _lib.stream_handle(device)), "ssa_paged_attention")
+                                                              int(not equal))
+    if need < 0:
+        raise ValueError("paged.attention: sizes out of range")
+    if len(_BYTES) >= 4096:
+        _BYTES.clear()
+    _BYTES[key] = need
+    return need
