@@ -397,15 +397,16 @@ __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, 
   float m = -INFINITY, ls = 0.0f;
   int hu = begin + (NW == 1 ? 0 : wave);
   PageList list(p, j, hu >> 1, lane);
+  // the query rows and the list, in a form the compiler counts: it does not
+  // know of the row loads to come, and would wait for the query rows in every
+  // step
+  wait_loads();
   Unit u{-1, 0};
   if (hu < end) {
     u = list.at(p, j, hu >> 1, lane);
     issue(kh, koff, u, hu, kb);
     issue(vh, voff, u, hu, vb);
   }
-  // everything so far, once and in a form the compiler counts: it does not
-  // know of the row loads, and would wait for the query rows in every step
-  wait_loads();
   for (; hu < end; hu += NW) {
     const bool more = hu + NW < end;
     loads_left<8>();                                        // K landed, V behind it
@@ -628,6 +629,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   const uint8_t* const kh = (const uint8_t*)(p.k + (long long)j.h * p.kv_head);
   const uint8_t* const vh = (const uint8_t*)(p.v + (long long)j.h * p.kv_head);
   PageList list(p, j, begin, lane);
+  wait_loads();       // as in narrow_tile
   int rows_ahead[kSlots] = {0, 0, 0, 0};    // rows of units i .. i + 3
   auto issue = [&](int u) {
     if (u >= end) return 0;
@@ -645,13 +647,23 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   f32x16 O[4], S;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
-  float m = -INFINITY, ls = 0.0f, nb, mx;
+  // the running maximum in log2 units; the exponents' offset and the raw score
+  // that the accumulators are rescaled beyond, which change with it alone
+  float m = -INFINITY, nb = kLift<F16>, beyond = -INFINITY, ls = 0.0f, mx;
+  const float slack = kSlack / p.scale_log2;
   const uint32_t klane = (uint32_t)(r * 256 + ((hh ^ (r & 15)) << 4));
   uint32_t vlane;
   {
     const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2);
     vlane = (uint32_t)(row * 256 + (((2 * (g & 1) + ((i & 3) >> 1)) ^ vswz(row)) << 4) + (i & 1) * 8);
   }
+  // addresses of the K and V operands in slot 0: the slots lie at instruction
+  // offsets, so that a step forms none (12 fewer vector instructions per half page)
+  const lds_u8 *kat[8], *vat[4];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) kat[x] = kring + (klane ^ (uint32_t)(x << 5));
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) vat[dt] = vring + (vlane ^ (uint32_t)(dt << 6));
   // rows of a page behind its end hold anything: 0 * NaN must not reach the
   // sums, so each wave clears those of its V rows once they have landed
   auto clear_rows = [&](int u, int rows) {
@@ -676,113 +688,118 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
 #pragma unroll
     for (int i = 0; i < 16; ++i) X[i] = 8 * (i / 4) + i % 4 < see ? X[i] : -INFINITY;
   };
+  // mx: the lane's row's maximum of the scores to come, as they are
   auto rescale = [&]() {
-    if (__any(mx > m + kSlack)) {
-      const float to = __builtin_fmaxf(m, mx);
-      const float a = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));
+    if (__any(mx > beyond)) {
+      const float to = __builtin_fmaxf(m, mx * p.scale_log2), at = to == -INFINITY ? 0.0f : to;
+      const float a = __builtin_amdgcn_exp2f(m - at);
       ls *= a;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
       m = to;
+      nb = kLift<F16> - at;
+      beyond = __builtin_fmaxf(beyond - slack, mx) + slack;
     }
-    nb = kLift<F16> - (m == -INFINITY ? 0.0f : m);
   };
-  // Half a page: the probabilities of Sc meet V (rows 32 half .. of `vb`), with
-  // the scores Sn of the next half page (rows of `kb`) and their maximum.  ka
-  // holds the first four K operands on entry, and on return those of the half
-  // page after (rows of `kafter`).
+  // Half a page: the probabilities of Sc meet V (rows 32 half .. of slot `slot`),
+  // with the scores Sn of the next half page and their maximum.  ka holds the
+  // first four K operands on entry, and on return those of the half page after.
+  // The scores' products run at raised priority: a wave in them keeps the pipe
+  // from the other one's sums, and the two fall out of step.
   u32x4 ka[8];
-  auto kread = [&](const lds_u8* kb, int x) { return *(lds_u32x4*)(kb + (klane ^ (uint32_t)(x << 5))); };
-  auto half_step = [&](const lds_u8* kb, const lds_u8* kafter, const lds_u8* vb, const f32x16& Sc, f32x16& Sn, int next,
-                       int next_half, int next_rows) {
+  auto kread = [&](int slot, int half, int x) {
+    return *(lds_u32x4*)(kat[x] + slot * kTile + half * (kTile / 2));
+  };
+  auto half_step = [&](auto slot_c, auto half_c, const f32x16& Sc, f32x16& Sn, int next, int next_rows) {
+    constexpr int slot = decltype(slot_c)::value, half = decltype(half_c)::value;
+    constexpr int nslot = (slot + half) % kSlots, nhalf = half ^ 1;            // the next half page
+    constexpr int aslot = (slot + 1) % kSlots, ahalf = half;                   // and the one after
     u32x4 va[2][4], pb[2];
-    float P[16], ps = 0.0f;
+    float P[16];
     auto vread = [&](int ks, int dt) {
-      const lds_u8* a = vb + 4096 * ks + (vlane ^ (uint32_t)(dt << 6));
+      const lds_u8* a = vat[dt] + slot * kTile + half * (kTile / 2) + 4096 * ks;
       return tr_pair(a, a + 2048);
     };
     auto expo = [&](int i) {
       P[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(Sc[i], p.scale_log2, nb));
-      ps += P[i];
+      ls += P[i];
       if (i & 1) pb[i >> 3][(i & 7) >> 1] = pack2<F16>(P[i - 1], P[i]);
     };
-    auto group = []() { __builtin_amdgcn_sched_barrier(0); };
     Sn = f32x16{};
-    group();
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int st = 0; st < 8; ++st) {
       Sn = mma<F16>(ka[st], qop[st], Sn);
       if (st < 4)
-        ka[st + 4] = kread(kb, st + 4);
+        ka[st + 4] = kread(nslot, nhalf, st + 4);
       else
         va[0][st - 4] = vread(0, st - 4);
       expo(st);
-      if (st & 1) expo(8 + st / 2);
-      group();
     }
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
       O[dt] = mma<F16>(va[0][dt], pb[0], O[dt]);
       va[1][dt] = vread(1, dt);
-      expo(12 + dt);
-      group();
+      expo(8 + 2 * dt);
+      expo(9 + 2 * dt);
     }
-    float part;
+    asm volatile("" : "+v"(ls));   // the sums here, not behind the branches below
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
       O[dt] = mma<F16>(va[1][dt], pb[1], O[dt]);
-      ka[dt] = kread(kafter, dt);
-      if (dt == 0) part = lane_max(Sn);
-      if (dt == 1) mx = half_max(part) * p.scale_log2;
-      if (dt == 2) {
-        ls += ps;
-        asm volatile("" : "+v"(ls));   // here, not behind the branches below
-      }
-      group();
+      ka[dt] = kread(aslot, ahalf, dt);
     }
-    if (cut(next, next_half, next_rows)) {
-      mask(Sn, next, next_half, next_rows);
-      mx = half_max(lane_max(Sn)) * p.scale_log2;
+    mx = half_max(lane_max(Sn));
+    if (cut(next, nhalf, next_rows)) {
+      mask(Sn, next, nhalf, next_rows);
+      mx = half_max(lane_max(Sn));
     }
     rescale();
   };
 
   if (begin < end) {
-    wait_loads();
+    if (begin + 3 <= end)
+      loads_left<6>();
+    else
+      loads_left<0>();
     clear_rows(begin, rows_ahead[0]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     S = f32x16{};
     if (alive) {
 #pragma unroll
-      for (int st = 0; st < 8; ++st) S = mma<F16>(kread(kring, st), qop[st], S);
+      for (int st = 0; st < 8; ++st) S = mma<F16>(kread(0, 0, st), qop[st], S);
     }
     if (cut(begin, 0, rows_ahead[0])) mask(S, begin, 0, rows_ahead[0]);
-    mx = half_max(lane_max(S)) * p.scale_log2;
+    mx = half_max(lane_max(S));
     rescale();
 #pragma unroll
-    for (int st = 0; st < 4; ++st) ka[st] = kread(kring + kTile / 2, st);
-    for (int u = begin; u < end; ++u) {
-      rows_ahead[3] = issue(u + 3);
-      const int slot = (u - begin) % kSlots, after = (u + 1 - begin) % kSlots;
-      const lds_u8 *k0 = kring + slot * kTile, *k1 = kring + after * kTile, *v = vring + slot * kTile;
+    for (int st = 0; st < 4; ++st) ka[st] = kread(0, 1, st);
+    int u = begin;
+    auto step = [&](auto slot_c) {
       f32x16 S1;
+      if (alive) half_step(slot_c, std::integral_constant<int, 0>{}, S, S1, u, rows_ahead[0]);
+      rows_ahead[3] = issue(u + 3);
       if (alive) {
-        half_step(k0 + kTile / 2, k1, v, S, S1, u, 1, rows_ahead[0]);
-        half_step(k1, k1 + kTile / 2, v + kTile / 2, S1, S, u + 1, 0, rows_ahead[1]);
+        half_step(slot_c, std::integral_constant<int, 1>{}, S1, S, u + 1, rows_ahead[1]);
       }
       // next: K of unit u + 2 and V of unit u + 1; each unit is 2 loads of K,
       // then 2 of V
       if (u + 3 < end)
-        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        loads_left<6>();
       else
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        loads_left<0>();
       rows_ahead[0] = rows_ahead[1];
       rows_ahead[1] = rows_ahead[2];
       rows_ahead[2] = rows_ahead[3];
       if (u + 1 < end) clear_rows(u + 1, rows_ahead[0]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
+      return ++u < end;
+    };
+    while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{}) &&
+           step(std::integral_constant<int, 2>{}) && step(std::integral_constant<int, 3>{})) {
     }
   }
 
