@@ -74,9 +74,9 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
                         float scale, int flags, void* workspace, long long workspace_bytes, hipStream_t stream);
 
 /* Bytes of that workspace (0: none needed), from sizes alone; -1 for sizes the
- * call rejects.  ragged: whether the call gives starts. */
+ * call rejects.  ragged: whether the call gives starts; causal: whether it is. */
 long long ssa_paged_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int prefix_tokens,
-                                              int table_pages, int ragged);
+                                              int table_pages, int ragged, int causal);
 
 #ifdef __cplusplus
 }

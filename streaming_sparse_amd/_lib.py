@@ -48,7 +48,7 @@ SIGNATURES = {
                          _vp, _vp, _ll, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "ssa_paged_attention": [_vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _i, _vp, _vp, _vp, _vp, _ll, _ll, _vp, _i, _i, _i,
                             _i, _i, _i, _f, _i, _vp, _ll, _vp],
-    "ssa_paged_attention_workspace_bytes": [_i, _i, _i, _i, _i, _i, _i],
+    "ssa_paged_attention_workspace_bytes": [_i, _i, _i, _i, _i, _i, _i, _i],
     "ssa_pset_noalloc": [_vp, _ll, _ll, _ll, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i,
                          _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
 }

@@ -19,7 +19,6 @@
 #include "../../include/ssattn_paged.h"
 
 #include <algorithm>
-#include <array>
 #include <cmath>
 #include <type_traits>
 
@@ -47,10 +46,13 @@ struct PagedParams {
   float scale_log2;
   // Work items of the launch: prefix_items of the prefix by itself
   // (prefix_tiles tiles per K/V head, of all sequences' rows, each in
-  // prefix_pieces pieces), then those of the sequences: own_tiles tiles per K/V
-  // head, the first own_whole of all heads' whole, the others in own_pieces
-  // pieces.  They walk the prefix too unless it is `apart`.
-  int prefix_items, prefix_tiles, prefix_pieces, own_tiles, own_whole, own_pieces, apart;
+  // prefix_pieces pieces of prefix_cut pages), then those of the sequences:
+  // own_tiles tiles per K/V head, the first own_whole of all heads' whole, the
+  // others in up to own_pieces pieces of own_cut pages.  They walk the prefix
+  // too unless it is `apart`.  longest_first (own_whole 0, or all): the tiles with
+  // the longest lists, a causal sequence's last, come first.
+  int prefix_items, prefix_tiles, prefix_pieces, prefix_cut, own_tiles, own_whole, own_pieces, own_cut, apart,
+      longest_first;
   int row_tiles;      // 32-row tiles of a K/V head's rows, where the prefix is apart
 };
 
@@ -142,10 +144,10 @@ __device__ __forceinline__ u32x4 tr_pair(const lds_u8* a, const lds_u8* b) {
 struct Job {
   int h;              // K/V head
   int rho0, rho1;     // rows
-  int piece, pieces;  // this piece of the list
   int state;          // where its states go, -1: it writes out
   int b, n, length, first_token;   // the rows' sequence: new tokens, rows in the cache, first packed token
   int prefix_pages, own_pages;     // pages of the list
+  int begin, end;                  // this piece of it
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -153,14 +155,20 @@ __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x,
 // Sequence and tile of the idx-th tile of T rows, sequence by sequence (each
 // sequence's last tile may be short); b = -1 behind the last.  One pass per 64
 // sequences: every lane counts one sequence's tiles, a wave scan sums them.
+// `last_first`: the last tile of each sequence first, and where the sequences
+// have equal counts the last tiles of all before the others.
 struct SeqTile {
   int b, tile, start, n;
 };
-__device__ __forceinline__ SeqTile find_tile(const PagedParams& p, int idx, int T, int lane) {
+__device__ __forceinline__ SeqTile find_tile(const PagedParams& p, int idx, int T, bool last_first, int lane) {
   if (!p.starts) {
-    const int each = (p.per_seq * p.group + T - 1) / T, b = idx / each;
-    if (b >= p.batch) return SeqTile{-1, 0, 0, 0};
-    return SeqTile{b, idx - b * each, b * p.per_seq, p.per_seq};
+    const int each = (p.per_seq * p.group + T - 1) / T;
+    if (last_first) {
+      const int level = idx / p.batch, b = idx - level * p.batch;
+      return SeqTile{level < each ? b : -1, each - 1 - level, b * p.per_seq, p.per_seq};
+    }
+    const int b = idx / each;
+    return SeqTile{b < p.batch ? b : -1, idx - b * each, b * p.per_seq, p.per_seq};
   }
   int base = 0;
   for (int c = 0; c < p.batch; c += 64) {
@@ -176,9 +184,10 @@ __device__ __forceinline__ SeqTile find_tile(const PagedParams& p, int idx, int 
     }
     const unsigned long long past = __ballot(base + sum > idx);
     if (past) {
-      const int l = __ffsll((long long)past) - 1;
-      const int before = base + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l);
-      return SeqTile{c + l, idx - before, __builtin_amdgcn_readlane(s0, l), __builtin_amdgcn_readlane(n, l)};
+      const int l = __ffsll((long long)past) - 1, count = __builtin_amdgcn_readlane(tiles, l);
+      const int tile = idx - (base + __builtin_amdgcn_readlane(sum, l) - count);
+      return SeqTile{c + l, last_first ? count - 1 - tile : tile, __builtin_amdgcn_readlane(s0, l),
+                     __builtin_amdgcn_readlane(n, l)};
     }
     base += __builtin_amdgcn_readlane(sum, 63);
   }
@@ -190,59 +199,71 @@ __device__ __forceinline__ int packed_tokens(const PagedParams& p) {
   return p.starts ? clampi(p.starts[p.batch], 0, p.tokens) : p.tokens;
 }
 
-// The rows of the idx-th own tile of T rows over all K/V heads; false: none.
+// Prefix item `item` of tiles of T rows; false: no rows.
 template <int T>
-__device__ __forceinline__ bool find_rows(const PagedParams& p, int idx, int lane, Job& j) {
-  j.h = idx / p.own_tiles;
-  const SeqTile s = find_tile(p, idx - j.h * p.own_tiles, T, lane);
-  if (s.b < 0) return false;
+__device__ __forceinline__ bool prefix_job(const PagedParams& p, int item, Job& j) {
+  const int tp = item / p.prefix_pieces;
+  j.state = item - tp * p.prefix_pieces;
+  j.h = tp / p.prefix_tiles;
+  j.rho0 = (tp - j.h * p.prefix_tiles) * T;
+  j.rho1 = min(j.rho0 + T, packed_tokens(p) * p.group);
+  j.b = 0;
+  j.n = j.length = j.first_token = 0;
+  j.prefix_pages = (p.prefix_tokens + kPage - 1) / kPage;
+  j.own_pages = 0;
+  j.begin = j.state * p.prefix_cut;
+  j.end = min(j.begin + p.prefix_cut, j.prefix_pages);
+  return j.rho0 < j.rho1;
+}
+
+// Own item `item` (behind the prefix items) of tiles of T rows; false: nothing
+// to do.
+template <int T>
+__device__ __forceinline__ bool own_job(const PagedParams& p, int item, int lane, Job& j) {
+  // the tile over all heads, and its piece
+  int idx = item, piece = 0, t;
+  if (p.longest_first) {
+    // the first pieces of all tiles, then the second ones, ...; the heads of a
+    // tile next to each other, so that with 8 heads an XCD keeps to one
+    const int all = p.kv_heads * p.own_tiles;
+    piece = item / all;
+    idx = item - piece * all;
+    t = idx / p.kv_heads;
+    j.h = idx - t * p.kv_heads;
+  } else {
+    if (item >= p.own_whole) {
+      const int u = (item - p.own_whole) / p.own_pieces;
+      piece = item - p.own_whole - u * p.own_pieces;
+      idx = p.own_whole + u;
+    }
+    j.h = idx / p.own_tiles;
+    t = idx - j.h * p.own_tiles;
+  }
+  const SeqTile s = find_tile(p, t, T, p.longest_first, lane);
+  if (s.b < 0 || s.tile < 0) return false;
   j.b = s.b;
   j.n = s.n;
   j.first_token = s.start;
   j.rho0 = s.start * p.group + s.tile * T;
   j.rho1 = min(j.rho0 + T, (s.start + s.n) * p.group);
-  return j.rho0 < j.rho1;
-}
-
-// Prefix item `item` of tiles of T rows; false: no rows.
-template <int T>
-__device__ __forceinline__ bool prefix_job(const PagedParams& p, int item, Job& j) {
-  const int tp = item / p.prefix_pieces;
-  j.piece = item - tp * p.prefix_pieces;
-  j.h = tp / p.prefix_tiles;
-  j.rho0 = (tp - j.h * p.prefix_tiles) * T;
-  j.rho1 = min(j.rho0 + T, packed_tokens(p) * p.group);
-  j.pieces = p.prefix_pieces;
-  j.state = j.piece;
-  j.b = 0;
-  j.n = j.length = j.first_token = 0;
-  j.prefix_pages = (p.prefix_tokens + kPage - 1) / kPage;
-  j.own_pages = 0;
-  return j.rho0 < j.rho1;
-}
-
-// Own item `item` (behind the prefix items) of tiles of T rows; false: no rows.
-template <int T>
-__device__ __forceinline__ bool own_job(const PagedParams& p, int item, int lane, Job& j) {
-  int tile = item;
-  j.piece = 0;
-  j.pieces = 1;
-  j.state = p.apart ? p.prefix_pieces : -1;
-  if (item >= p.own_whole) {
-    const int i = item - p.own_whole, t = i / p.own_pieces;
-    j.piece = i - t * p.own_pieces;
-    j.pieces = p.own_pieces;
-    j.state = p.apart ? p.prefix_pieces + j.piece : p.own_pieces > 1 ? i : -1;
-    tile = p.own_whole + t;
-  }
-  if (!find_rows<T>(p, tile, lane, j)) return false;
+  if (j.rho0 >= j.rho1) return false;
   j.length = clampi(p.lengths[j.b], 0, kPage * p.table_pages);
   j.prefix_pages = p.apart ? 0 : (p.prefix_tokens + kPage - 1) / kPage;
   // rows the tile's last query sees
   int seen = j.length;
   if (p.causal) seen = clampi(j.length - j.n + (j.rho1 - 1) / p.group - j.first_token + 1, 0, j.length);
   j.own_pages = (seen + kPage - 1) / kPage;
-  return true;
+  const int units = j.prefix_pages + j.own_pages;
+  const int cut = item < p.own_whole || p.own_pieces == 1 ? max(units, 1) : p.own_cut;
+  j.begin = min(piece * cut, units);
+  j.end = min(j.begin + cut, units);
+  if (p.apart) {
+    j.state = p.prefix_pieces + piece;       // a piece without pages leaves an empty state
+    return true;
+  }
+  // a list that fits one piece is written out by it
+  j.state = units > cut ? (idx - p.own_whole) * p.own_pieces + piece : -1;
+  return piece == 0 || j.begin < units;
 }
 
 // The state that holds row rho (block `blk` of a tile of T rows) of a job, and
@@ -322,8 +343,9 @@ __device__ __forceinline__ void finish_row(const PagedParams& p, const Job& j, c
   if (j.state >= 0) {
     int col;
     float* st = state_of<T>(p, j, rho, blk, &col);
+    // the sums of an empty state are not read
 #pragma unroll
-    for (int c = 0; c < 16; ++c) {
+    for (int c = 0; c < 16 && j.begin < j.end; ++c) {
       const f32x16& o = O[c >> 2];
       const int i = 4 * (c & 3);
       *reinterpret_cast<f32x4*>(st + ((2 * c + hh) * 32 + col) * 4) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
@@ -363,10 +385,7 @@ __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, 
   }
   const int all_see = __builtin_amdgcn_readfirstlane(limit);
 
-  // half pages [begin, end) of the list
-  const int units = j.prefix_pages + j.own_pages;
-  const int begin = 2 * (int)((long long)units * j.piece / j.pieces);
-  const int end = 2 * (int)((long long)units * (j.piece + 1) / j.pieces);
+  const int begin = 2 * j.begin, end = 2 * j.end;      // half pages
 
   // per-lane byte offsets of 16 rows' loads (instruction form: load jj leaves
   // out the 1024 jj that its offset field adds)
@@ -610,9 +629,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   // loads
   const int all_see = __builtin_amdgcn_readfirstlane(limit);
   const bool alive = j.rho0 + 32 * wave < j.rho1;
-  const int units = j.prefix_pages + j.own_pages;
-  const int begin = (int)((long long)units * j.piece / j.pieces);
-  const int end = (int)((long long)units * (j.piece + 1) / j.pieces);
+  const int begin = j.begin, end = j.end;
 
   lds_u8* const kring = ring;
   lds_u8* const vring = kring + kSlots * kTile;
@@ -817,8 +834,10 @@ __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p)
   static_assert(sizeof(ring) >= kWideWaves * 2 * kHalf);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int b = blockIdx.x, first = APART ? p.prefix_items : p.own_whole;
-  // the longer items first; either kind by itself over the XCDs
-  const int item = b < first ? xcd_remap(b, first) : xcd_remap(b - first, gridDim.x - first);
+  // the longer items first; either kind by itself over the XCDs, but for tiles in
+  // the order of their lists
+  int item = b < first ? b : b - first;
+  if (APART || !p.longest_first) item = xcd_remap(item, b < first ? first : gridDim.x - first);
   Job j;
   if constexpr (APART) {
     if (b < first) {
@@ -834,16 +853,72 @@ __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p)
   }
 }
 
-// Joins the pieces' states of 32 rows of a K/V head, dims 32 dt ..: block (h, rows
-// 32 T .., dt) where the prefix is apart (T_ROWS 0), else (split tile of T_ROWS
-// rows, block of 32, dt); wave w takes dims 8 w .. 8 w + 7.  Bound by the latency
-// of its loads: those of 8 pieces are out together.
-constexpr int kJoin = 8;
+// What a lane gathers of the pieces c, c + stride, ... of a row: M, L and N groups
+// of 4 dims, `at` floats into a state; kJoin pieces' loads are out together.
+constexpr int kJoin = 8, kJoinWaves = 4;
 
-template <bool F16, int T_ROWS>
-__global__ __launch_bounds__(256) void join_kernel(PagedParams p) {
+template <int N>
+struct Gathered {
+  float M = -INFINITY, L = 0.0f;
+  f32x4 o[N];
+};
+
+template <int N, int STEP>
+__device__ __forceinline__ Gathered<N> gather(const float* st, long long step, int first, int pieces, int stride, int r,
+                                              int at, bool live) {
+  Gathered<N> got;
+#pragma unroll
+  for (int x = 0; x < N; ++x) got.o[x] = f32x4{};
+  for (int c = first; c < pieces; c += kJoin * stride) {
+    float m[kJoin], l[kJoin];
+    f32x4 o[kJoin][N];
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < N; ++x) o[i][x] = f32x4{};
+      if (c + i * stride < pieces && live) {
+        const float* s = st + (c + i * stride) * step;
+        m[i] = s[32 * kHeadDim + r];
+        l[i] = s[32 * kHeadDim + 32 + r];
+#pragma unroll
+        for (int x = 0; x < N; ++x) o[i][x] = *reinterpret_cast<const f32x4*>(s + at + x * STEP);
+      }
+    }
+    float top = got.M;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) top = __builtin_fmaxf(top, m[i]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    const float a = __builtin_amdgcn_exp2f(got.M - ref);
+    got.L *= a;
+#pragma unroll
+    for (int x = 0; x < N; ++x) got.o[x] *= a;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      const float w = __builtin_amdgcn_exp2f(m[i] - ref);
+      got.L += l[i] * w;
+      // an empty state's sums are not there
+#pragma unroll
+      for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) got.o[x][k] += m[i] == -INFINITY ? 0.0f : o[i][x][k] * w;
+    }
+    got.M = top;
+  }
+  return got;
+}
+
+// Joins the pieces' states of 32 rows of a K/V head: block (h, rows 32 T .., group)
+// where the prefix is apart (T_ROWS 0), else (split tile of T_ROWS rows, block of
+// 32, group).  Bound by the latency of its loads.  Few pieces: a group is 32 dims, a
+// wave gathers 8 of them over all pieces.  MANY: a group is 16 dims, which the
+// four waves gather over a quarter of the pieces each; their sums meet in LDS.
+template <bool F16, int T_ROWS, bool MANY>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedParams p) {
+  constexpr int kGroups = MANY ? 8 : 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int dt = blockIdx.x & 3, block = blockIdx.x >> 2, r = lane & 31, hh = lane >> 5;
+  const int g = blockIdx.x % kGroups, block = blockIdx.x / kGroups, r = lane & 31, hh = lane >> 5;
   int h, rho, end, pieces;
   long long step;                 // floats from a piece to the next
   const float* st;
@@ -858,60 +933,66 @@ __global__ __launch_bounds__(256) void join_kernel(PagedParams p) {
     constexpr int kBlocks = T_ROWS / 32;
     const int t = block / kBlocks, blk = block - t * kBlocks;
     Job j;
-    if (!find_rows<T_ROWS>(p, p.own_whole + t, lane, j)) return;
+    // the tile's first piece
+    if (!own_job<T_ROWS>(p, p.longest_first ? t : p.own_whole + t * p.own_pieces, lane, j) || j.state < 0) return;
     h = j.h;
     rho = j.rho0 + 32 * blk + r;
     end = j.rho1;
-    pieces = p.own_pieces;
+    pieces = (j.prefix_pages + j.own_pages + p.own_cut - 1) / p.own_cut;
     step = (long long)kBlocks * kState;
-    st = p.part + ((long long)t * pieces * kBlocks + blk) * kState;
+    st = p.part + ((long long)t * p.own_pieces * kBlocks + blk) * kState;
   }
   const bool live = rho < end;
-  float M = -INFINITY, L = 0.0f;
-  f32x4 acc = {};
-  for (int c = 0; c < pieces; c += kJoin, st += kJoin * step) {
-    float m[kJoin], l[kJoin];
-    f32x4 o[kJoin];
-#pragma unroll
-    for (int i = 0; i < kJoin; ++i) {
-      m[i] = -INFINITY;
-      l[i] = 0.0f;
-      o[i] = f32x4{};
-      if (c + i < pieces && live) {
-        m[i] = st[i * step + 32 * kHeadDim + r];
-        l[i] = st[i * step + 32 * kHeadDim + 32 + r];
-        o[i] = *reinterpret_cast<const f32x4*>(st + i * step + ((8 * dt + 2 * wave + hh) * 32 + r) * 4);
-      }
+  float M, L;
+  f32x4 o;
+  int dims;
+  if constexpr (MANY) {
+    __shared__ f32x4 xo[kJoinWaves][2][64];
+    __shared__ float xm[kJoinWaves][32], xl[kJoinWaves][32];
+    const Gathered<2> got =
+        gather<2, 256>(st, step, wave, pieces, kJoinWaves, r, ((4 * g + hh) * 32 + r) * 4, live);
+    if (hh == 0) {
+      xm[wave][r] = got.M;
+      xl[wave][r] = got.L;
     }
-    float top = M;
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i) top = __builtin_fmaxf(top, m[i]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    const float a = __builtin_amdgcn_exp2f(M - ref);
-    acc *= a;
-    L *= a;
+    for (int x = 0; x < 2; ++x) xo[wave][x][lane] = got.o[x];
+    __syncthreads();
+    if (wave >= 2) return;              // waves 0 and 1 finish 8 dims each
+    M = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i) {
-      const float w = __builtin_amdgcn_exp2f(m[i] - ref);
-      L += l[i] * w;
-      acc += o[i] * w;
+    for (int w = 0; w < kJoinWaves; ++w) M = __builtin_fmaxf(M, xm[w][r]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    L = 0.0f;
+    o = f32x4{};
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) {
+      const float a = __builtin_amdgcn_exp2f(xm[w][r] - ref);
+      L += xl[w][r] * a;
+      o += xo[w][wave][lane] * a;
     }
-    M = top;
+    dims = 16 * g + 8 * wave + 4 * hh;
+  } else {
+    const Gathered<1> got = gather<1, 0>(st, step, 0, pieces, 1, r, ((8 * g + 2 * wave + hh) * 32 + r) * 4, live);
+    M = got.M;
+    L = got.L;
+    o = got.o[0];
+    dims = 32 * g + 8 * wave + 4 * hh;
   }
   if (!live) return;
   const int token = rho / p.group, hq = h * p.group + rho % p.group;
   const bool none = __float_as_uint(L) == 0u;
-  acc *= none ? 0.0f : 1.0f / L;
-  *reinterpret_cast<u32x2*>(p.out + (long long)token * p.o_tok + (long long)hq * p.o_head + 32 * dt + 8 * wave + 4 * hh) =
-      u32x2{pack2<F16>(acc[0], acc[1]), pack2<F16>(acc[2], acc[3])};
-  if (p.lse && dt == 0 && wave == 0 && hh == 0)
-    p.lse[(long long)token * p.heads + hq] = lse_of(M, L);
+  o *= none ? 0.0f : 1.0f / L;
+  *reinterpret_cast<u32x2*>(p.out + (long long)token * p.o_tok + (long long)hq * p.o_head + dims) =
+      u32x2{pack2<F16>(o[0], o[1]), pack2<F16>(o[2], o[3])};
+  if (p.lse && dims == 0) p.lse[(long long)token * p.heads + hq] = lse_of(M, L);
 }
 
 // How a call is cut up, from sizes alone.  Tiles are of 32 rows (narrow) or 256
 // (wide); own tiles beside prefix tiles are narrow.
 struct Plan {
-  int rows, row_tiles, prefix_tiles, prefix_pieces, own_tiles, own_whole, own_pieces;
+  int rows, row_tiles, prefix_tiles, prefix_pieces, prefix_cut, own_tiles, own_whole, own_pieces, own_cut;
+  bool longest_first;
   bool apart() const { return prefix_tiles > 0; }
   long long split_tiles(int kv_heads) const { return (long long)kv_heads * own_tiles - own_whole; }
   long long states(int kv_heads) const {
@@ -928,7 +1009,7 @@ double wide_page(double rows) { return 1.0 + 0.9 * std::min(1.0, rows / kWide); 
 double state_time(double rows) { return rows * 2 * (4.0 * kState / 32) / 4.5e6; }
 double page_time(double pages) { return pages * 32768 / 5.2e6; }
 
-constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64};
+constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64, 96, 128, 192, 256};
 
 // When n workgroups of the time t each, and then m of the time u, are done on
 // `slots` places.
@@ -946,105 +1027,132 @@ bool sizes_fit(int tokens, int batch, int heads, int kv_heads, int prefix_tokens
          (long long)table_pages * kPage < (1ll << 30) && prefix_tokens < (1 << 30) && batch <= (1 << 20);
 }
 
-// Tiles over all heads of T rows, of sequences by themselves.
-int seq_tiles(long long rows, int batch, bool ragged, int T) {
-  return (int)(ragged ? rows / T + batch : (long long)batch * ((rows / batch + T - 1) / T));
+// `units` pages in about c pieces of *cut; returns how many.
+int cut_in(int units, int c, int* cut) {
+  *cut = (units + c - 1) / c;
+  return (units + *cut - 1) / *cut;
 }
+
+// The sizes that a plan goes by.
+struct Sizes {
+  int cus, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, ragged, causal;
+  bool operator==(const Sizes& o) const {
+    return cus == o.cus && tokens == o.tokens && batch == o.batch && heads == o.heads && kv_heads == o.kv_heads &&
+           prefix_tokens == o.prefix_tokens && table_pages == o.table_pages && ragged == o.ragged &&
+           causal == o.causal;
+  }
+  int prefix_pages() const { return (prefix_tokens + kPage - 1) / kPage; }
+  long long rows() const { return (long long)tokens * (heads / kv_heads); }     // of a K/V head
+  // tiles of T rows of a K/V head, of sequences by themselves, at most
+  int seq_tiles(int T) const {
+    return (int)(ragged ? rows() / T + batch : batch * ((rows() / batch + T - 1) / T));
+  }
+};
 
 // The prefix apart: all rows together over the prefix, each sequence over its own
 // pages.  Returns the estimated time.
-double plan_apart(int cus, long long rows, int batch, int kv_heads, int prefix_pages, int table_pages, bool ragged,
-                  Plan* plan) {
-  const int T = rows <= kNarrow ? kNarrow : kWide;
+double plan_apart(const Sizes& z, Plan* plan) {
+  const long long rows = z.rows();
+  const int T = rows <= kNarrow ? kNarrow : kWide, prefix_pages = z.prefix_pages();
   const bool wide = T == kWide;
-  const int slots = wide ? cus : 2 * cus, waves = wide ? kWideWaves : kNarrowWaves;
+  const int slots = wide ? z.cus : 2 * z.cus, waves = wide ? kWideWaves : kNarrowWaves;
   plan->rows = T;
   plan->row_tiles = (int)((rows + 31) / 32);
   plan->prefix_tiles = (int)((rows + T - 1) / T);
-  plan->own_tiles = seq_tiles(rows, batch, ragged, kNarrow);
+  plan->own_tiles = z.seq_tiles(kNarrow);
   plan->own_whole = 0;
-  const double tiles = (double)kv_heads * plan->prefix_tiles, own_tiles = (double)kv_heads * plan->own_tiles;
+  plan->longest_first = false;
+  const double tiles = (double)z.kv_heads * plan->prefix_tiles, own_tiles = (double)z.kv_heads * plan->own_tiles;
   const double page = wide ? wide_page((double)rows / plan->prefix_tiles) : kNarrowPage;
-  const double floor_time = page_time(kv_heads * (prefix_pages + 0.6 * batch * table_pages));
+  const double floor_time = page_time(z.kv_heads * (prefix_pages + 0.6 * z.batch * z.table_pages));
   double least = 1e30;
   for (int c : kCuts) {
     if (c > 1 && 2 * c > prefix_pages) break;
-    const double t = kStart + (prefix_pages + c - 1) / c * page;
+    int cut;
+    const int pieces = cut_in(prefix_pages, c, &cut);
+    const double t = kStart + cut * page;
     for (int d : kCuts) {
-      if (d > 16 || (d > 1 && 2 * d > table_pages)) break;
-      const double u = kStart + (table_pages + d - 1) / d * kSoloPage;
-      const double cost = std::max(floor_time, makespan(tiles * c, t, own_tiles * d / waves, u, slots)) +
-                          state_time((double)kv_heads * rows * (c + d)) + kJoinStart;
+      if (d > 16 || (d > 1 && 2 * d > z.table_pages)) break;
+      int own_cut;
+      const int own = cut_in(z.table_pages, d, &own_cut);
+      const double u = kStart + own_cut * kSoloPage;
+      const double cost = std::max(floor_time, makespan(tiles * pieces, t, own_tiles * own / waves, u, slots)) +
+                          state_time((double)z.kv_heads * rows * (pieces + own)) + kJoinStart;
       if (cost < least) {
         least = cost;
-        plan->prefix_pieces = c;
-        plan->own_pieces = d;
+        plan->prefix_pieces = pieces;
+        plan->prefix_cut = cut;
+        plan->own_pieces = own;
+        plan->own_cut = own_cut;
       }
     }
   }
   return least;
 }
 
-// Every tile over prefix and own pages.  With more wide tiles than CUs, only
-// those behind the last full round are cut.
-double plan_joint(int cus, long long rows, int batch, int kv_heads, int prefix_pages, int table_pages, bool ragged,
-                  Plan* plan) {
-  const double per_seq = (double)rows / batch;
-  const int T = per_seq <= kNarrow ? kNarrow : kWide;
+// Every tile over prefix and own pages.  Where their lists are alike and there
+// are more wide tiles than CUs, only those behind the last full round are cut;
+// where a causal sequence's first tiles have much shorter lists than its last,
+// every list is cut at the same length.
+double plan_joint(const Sizes& z, Plan* plan) {
+  const double per_seq = (double)z.rows() / z.batch;
+  const int T = per_seq <= kNarrow ? kNarrow : kWide, units = z.table_pages + z.prefix_pages();
   const bool wide = T == kWide;
-  const int slots = wide ? cus : 2 * cus;
+  const int slots = wide ? z.cus : 2 * z.cus;
   plan->rows = T;
-  plan->row_tiles = plan->prefix_tiles = plan->prefix_pieces = 0;
-  plan->own_tiles = seq_tiles(rows, batch, ragged, T);
-  const long long own_tiles = (long long)kv_heads * plan->own_tiles, whole = wide ? own_tiles / cus * cus : 0;
-  const int units = table_pages + prefix_pages;
+  plan->row_tiles = plan->prefix_tiles = plan->prefix_pieces = plan->prefix_cut = 0;
+  plan->own_tiles = z.seq_tiles(T);
+  // pages that the first tile of a sequence sees fewer of than the last
+  const double spread = z.causal ? (double)(z.tokens / z.batch) / kPage : 0.0;
+  plan->longest_first = wide && spread > 0.2 * units;
+  const long long own_tiles = (long long)z.kv_heads * plan->own_tiles;
+  const long long whole = wide && !plan->longest_first ? own_tiles / z.cus * z.cus : 0;
   const double tiles = (double)(own_tiles - whole);
   const double live = per_seq / std::ceil(per_seq / T);     // rows of a tile that there are
   const double page = wide ? wide_page(live) : kNarrowPage;
   double least = tiles > 0 ? 1e30 : 0.0;
   plan->own_pieces = 1;
+  plan->own_cut = units;
   for (int c : kCuts) {
     if (tiles == 0 || (c > 1 && 2 * c > units)) break;
-    const int pages = (units + c - 1) / c;
-    const double rounds = std::ceil(tiles * c / slots);
-    const double cost = rounds * std::max(kStart + pages * page, page_time(std::min(tiles * c, (double)slots) * pages)) +
-                        (c > 1 ? state_time(tiles * c * live) + kJoinStart : 0.0);
+    int cut;
+    const int pieces = cut_in(units, c, &cut);
+    const double longest = kStart + cut * page;
+    double time, states = 0.0;
+    if (plan->longest_first) {
+      const double mean = units - 0.5 * spread, each = std::max(1.0, mean / cut + (c > 1 ? 0.5 : 0.0));
+      time = tiles * each <= slots ? longest
+                                   : std::max(longest, tiles * (each * kStart + mean * page) / slots + 0.5 * longest);
+      states = c > 1 ? tiles * each : 0.0;
+    } else {
+      time = std::ceil(tiles * pieces / slots) * std::max(longest, page_time(std::min(tiles * pieces, (double)slots) * cut));
+      states = pieces > 1 ? tiles * pieces : 0.0;
+    }
+    const double cost = time + (states > 0 ? state_time(states * live) + kJoinStart : 0.0);
     if (cost < least) {
       least = cost;
-      plan->own_pieces = c;
+      plan->own_pieces = pieces;
+      plan->own_cut = cut;
     }
   }
   plan->own_whole = (int)(plan->own_pieces == 1 ? own_tiles : whole);
-  return least + (double)(whole / cus) * (kStart + units * page);
+  return least + (double)(whole / z.cus) * (kStart + units * page);
 }
 
-// The plan of a call's sizes.  A thread keeps its last one: the estimates of all
-// cuts take longer than a launch.
-int make_plan(int tokens, int batch, int heads, int kv_heads, int prefix_tokens, int table_pages, bool ragged,
-              Plan* plan) {
-  int cus = 0;
-  const int e = device_cus(&cus);
+// The plan of a call's sizes (z.cus is filled in).  A thread keeps its last one:
+// the estimates of all cuts take longer than a launch.
+int make_plan(Sizes z, Plan* plan) {
+  const int e = device_cus(&z.cus);
   if (e != (int)hipSuccess) return e;
-  struct Last {
-    std::array<int, 8> sizes{};
-    Plan plan;
-  };
-  static thread_local Last last;
-  const std::array<int, 8> sizes = {cus, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, (int)ragged};
-  if (sizes == last.sizes) {
-    *plan = last.plan;
-    return (int)hipSuccess;
+  static thread_local Sizes last_sizes{};
+  static thread_local Plan last_plan;
+  if (!(z == last_sizes)) {
+    Plan joint, apart;
+    const double t = plan_joint(z, &joint);
+    last_plan = z.batch > 1 && z.prefix_tokens > 0 && plan_apart(z, &apart) < t ? apart : joint;
+    last_sizes = z;
   }
-  const long long rows = (long long)tokens * (heads / kv_heads);
-  const int prefix_pages = (prefix_tokens + kPage - 1) / kPage;
-  const double joint = plan_joint(cus, rows, batch, kv_heads, prefix_pages, table_pages, ragged, plan);
-  if (batch > 1 && prefix_pages > 0) {
-    Plan other;
-    const double apart = plan_apart(cus, rows, batch, kv_heads, prefix_pages, table_pages, ragged, &other);
-    if (apart < joint) *plan = other;
-  }
-  last.sizes = sizes;
-  last.plan = *plan;
+  *plan = last_plan;
   return (int)hipSuccess;
 }
 
@@ -1053,10 +1161,11 @@ int make_plan(int tokens, int batch, int heads, int kv_heads, int prefix_tokens,
 extern "C" {
 
 long long ssa_paged_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int prefix_tokens,
-                                              int table_pages, int ragged) {
+                                              int table_pages, int ragged, int causal) {
   Plan plan;
   if (!sizes_fit(tokens, batch, heads, kv_heads, prefix_tokens, table_pages, ragged != 0) ||
-      make_plan(tokens, batch, heads, kv_heads, prefix_tokens, table_pages, ragged != 0, &plan) != (int)hipSuccess)
+      make_plan(Sizes{0, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, ragged != 0, causal != 0}, &plan) !=
+          (int)hipSuccess)
     return -1;
   return plan.bytes(kv_heads);
 }
@@ -1079,7 +1188,8 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
       (((uintptr_t)q | (uintptr_t)cache_k | (uintptr_t)cache_v | (uintptr_t)out) & 15) || ((uintptr_t)lse & 3))
     return (int)hipErrorInvalidValue;
   Plan plan;
-  const int e = make_plan(tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr, &plan);
+  const int e = make_plan(Sizes{0, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr,
+                                (flags & 2) != 0}, &plan);
   if (e != (int)hipSuccess) return e;
   const long long need = plan.bytes(kv_heads);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
@@ -1115,9 +1225,12 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   p.row_tiles = plan.row_tiles;
   p.prefix_tiles = plan.prefix_tiles;
   p.prefix_pieces = plan.prefix_pieces;
+  p.prefix_cut = plan.prefix_cut;
   p.own_tiles = plan.own_tiles;
   p.own_whole = plan.own_whole;
   p.own_pieces = plan.own_pieces;
+  p.own_cut = plan.own_cut;
+  p.longest_first = plan.longest_first;
   p.apart = plan.apart();
   const long long prefix_items = 1ll * kv_heads * plan.prefix_tiles * plan.prefix_pieces;
   const bool wide = plan.rows == kWide;
@@ -1126,8 +1239,9 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   const int waves = wide ? kWideWaves : kNarrowWaves;
   if (plan.apart()) own_items = (own_items + waves - 1) / waves;    // a wave each
   const long long items = prefix_items + own_items;
-  const long long joins = plan.apart() ? 4ll * kv_heads * plan.row_tiles
-                                       : plan.own_pieces > 1 ? plan.split_tiles(kv_heads) * (plan.rows / 8) : 0;
+  const bool many = plan.prefix_pieces + plan.own_pieces > kJoin;
+  const long long joins = (many ? 8 : 4) * (plan.apart() ? 1ll * kv_heads * plan.row_tiles
+                                            : plan.own_pieces > 1 ? plan.split_tiles(kv_heads) * (plan.rows / 32) : 0);
   if (items > 0x7fffffffll || joins > 0x7fffffffll) return (int)hipErrorInvalidValue;
   p.prefix_items = (int)prefix_items;
   const bool f16 = flags & 1;
@@ -1145,13 +1259,22 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   else
     start(narrow_kernel<true, true>, narrow_kernel<false, true>, narrow_kernel<true, false>,
           narrow_kernel<false, false>);
+  auto join = [&](auto f16_few, auto bf16_few, auto f16_many, auto bf16_many) {
+    if (many)
+      f16 ? launch(f16_many, joins, 64 * kJoinWaves) : launch(bf16_many, joins, 64 * kJoinWaves);
+    else
+      f16 ? launch(f16_few, joins, 64 * kJoinWaves) : launch(bf16_few, joins, 64 * kJoinWaves);
+  };
   if (joins > 0) {
     if (plan.apart())
-      f16 ? launch(join_kernel<true, 0>, joins, 256) : launch(join_kernel<false, 0>, joins, 256);
+      join(join_kernel<true, 0, false>, join_kernel<false, 0, false>, join_kernel<true, 0, true>,
+           join_kernel<false, 0, true>);
     else if (!wide)
-      f16 ? launch(join_kernel<true, kNarrow>, joins, 256) : launch(join_kernel<false, kNarrow>, joins, 256);
+      join(join_kernel<true, kNarrow, false>, join_kernel<false, kNarrow, false>, join_kernel<true, kNarrow, true>,
+           join_kernel<false, kNarrow, true>);
     else
-      f16 ? launch(join_kernel<true, kWide>, joins, 256) : launch(join_kernel<false, kWide>, joins, 256);
+      join(join_kernel<true, kWide, false>, join_kernel<false, kWide, false>, join_kernel<true, kWide, true>,
+           join_kernel<false, kWide, true>);
   }
   return (int)hipGetLastError();
 }

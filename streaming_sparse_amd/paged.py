@@ -247,7 +247,7 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
             raise ValueError("out must have q's shape")
     lse = workspace.tensor('paged_lse', (n, h), device, torch.float32) if want_lse else None
     if n:
-        key = (n, batch, h, g, prefix_tokens, width, starts is None, dev)
+        key = (n, batch, h, g, prefix_tokens, width, starts is None, causal, dev)
         need = _BYTES.get(key)
         if need is None:
             need = _workspace_bytes(key, device)
@@ -262,12 +262,12 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
 def _workspace_bytes(key, device):
     """The workspace that a call of these sizes needs, asked of the library once
     per sizes and device."""
-    tokens, batch, heads, kv_heads, prefix_tokens, width, equal, dev = key
+    tokens, batch, heads, kv_heads, prefix_tokens, width, equal, causal, dev = key
     if dev < 0:
         raise RuntimeError("the tensors must be on a GPU")
     with torch.cuda.device(device):
         need = _lib.lib().ssa_paged_attention_workspace_bytes(tokens, batch, heads, kv_heads, prefix_tokens, width,
-                                                              int(not equal))
+                                                              int(not equal), int(bool(causal)))
     if need < 0:
         raise ValueError("paged.attention: sizes out of range")
     if len(_BYTES) >= 4096:

@@ -155,7 +155,7 @@ def test_attention_abi_rejects():
                    dict(o_tok=-8), dict(tokens=1 << 30, batch=1 << 10), dict(width=1 << 26), dict(kv_tok=1 << 24)):
         assert attention_call(**change) == INVALID, change
     size = _lib.lib().ssa_paged_attention_workspace_bytes
-    assert size(3, 2, 4, 2, 0, 1, 0) == -1 and size(2, 2, 4, 3, 0, 1, 0) == -1 and size(0, 1, 1, 1, 0, 1, 0) == -1
+    assert size(3, 2, 4, 2, 0, 1, 0, 1) == -1 and size(2, 2, 4, 3, 0, 1, 0, 1) == -1 and size(0, 1, 1, 1, 0, 1, 0, 1) == -1
 
 
 def test_oracle_attention_is_dense_attention():
