@@ -1023,7 +1023,7 @@ double makespan(double n, double t, double m, double u, double slots) {
 
 bool sizes_fit(int tokens, int batch, int heads, int kv_heads, int prefix_tokens, int table_pages, bool ragged) {
   return tokens > 0 && batch > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && prefix_tokens >= 0 &&
-         table_pages > 0 && (ragged || tokens % batch == 0) && (long long)tokens * heads < (1ll << 31) &&
+         table_pages > 0 && (ragged || tokens % batch == 0) && (long long)tokens * heads < (1ll << 30) &&
          (long long)table_pages * kPage < (1ll << 30) && prefix_tokens < (1 << 30) && batch <= (1 << 20);
 }
 

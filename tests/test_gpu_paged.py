@@ -198,6 +198,73 @@ def test_attention_nan_and_inf_reach_only_who_sees_them(device):
     assert torch.isnan(out[0]).all() and torch.isfinite(out[1]).all()
 
 
+def test_attention_masked_nan_key(device):
+    """Keys of later tokens are masked whatever they hold: with NaN keys in the
+    last two tokens the earlier rows stay as they are."""
+    for new, before in (([7], [60]), ([300], [5])):
+        c = Case(device, new, before, 2, 2, 70)
+        want, _ = c.attend()
+        want = want.clone()
+        for at in (c.lengths[0] - 1, c.lengths[0] - 2):
+            c.k[0, 64 * int(c.table[0, int(at) // 64]) + int(at) % 64] = math.nan
+        got, _ = c.attend()
+        assert torch.equal(got[:c.N - 2], want[:c.N - 2]) and torch.isnan(got[c.N - 2:]).all()
+
+
+def test_attention_layouts(device):
+    """K and V side by side in one cache, head-major and broadcast queries, out in
+    place of q, a table whose entries behind the sequence are garbage."""
+    c = Case(device, [5, 40], [100, 3], 4, 2, 200, width=9)
+    want, want_lse = c.attend()
+    want, want_lse = want.clone(), want_lse.clone()
+    both = torch.stack([c.k[0], c.v[0]], 1)[None]
+    c.k, c.v = both[:, :, 0], both[:, :, 1]
+    used = -(-c.lengths // 64)
+    c.table[torch.arange(9, device=device) >= used[:, None]] = 0x7fffffff
+    c.q = c.q.transpose(0, 1).contiguous().transpose(0, 1)
+    got, lse = c.attend()
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    got, lse = c.attend(out=c.q)
+    assert got is c.q and torch.equal(got, want) and torch.equal(lse, want_lse)
+    one = c.wide[:1, :1].expand(c.N, c.H, 128)
+    c.q = one
+    a = c.attend()[0].clone()
+    c.q = one.contiguous()
+    assert torch.equal(c.attend()[0], a)
+
+
+def test_attention_no_rows_at_all(device):
+    """Every sequence brings no token: nothing is written, in either form of
+    call."""
+    for new in ([0, 0, 0], [0]):
+        c = Case(device, new, [70] * len(new), 2, 1, 90, padding=9)
+        out = torch.full_like(c.q, 5.0)
+        got, _ = c.attend(out=out)
+        assert (got == 5.0).all()
+
+
+def test_attention_many_ragged_sequences(device):
+    """More sequences than a wave scans at once, empty ones among them."""
+    new = [(7 * i) % 5 for i in range(150)]
+    c = Case(device, new, [(13 * i) % 90 for i in range(150)], 2, 1, 33)
+    c.check(*c.attend())
+
+
+def test_attention_two_streams_at_once(device):
+    """Two calls in flight together, each with a workspace of its own."""
+    cs = [Case(device, [1] * 12, [50 * i for i in range(12)], 8, 2, 3000, seed=s) for s in (1, 2)]
+    want = [tuple(x.clone() for x in c.attend()) for c in cs]
+    torch.cuda.synchronize()
+    streams, ws, got = [torch.cuda.Stream() for _ in cs], [Workspace() for _ in cs], [None, None]
+    for _ in range(10):
+        for i, c in enumerate(cs):
+            with torch.cuda.stream(streams[i]):
+                got[i] = c.attend(ws=ws[i])
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
 def append_case(device, c, k, v, **more):
     q = c.q
     ck, cv = c.k.clone(), c.v.clone()

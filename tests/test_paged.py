@@ -61,7 +61,10 @@ def test_append_rejects_bad_arguments():
     bad(freqs=a['f'], positions=torch.zeros(6, dtype=torch.int64))
     bad(positions=torch.zeros(6, dtype=torch.int32))
     bad(q_out=a['q'][:5])
+    bad(q_out=a['q'][:, :1].expand(6, 4, 128))               # written rows must not overlap
     bad(q=None, q_out=a['q'])
+    bad(ck=a['ck'][:, :, :1].expand(1, 384, 2, 128), cv=a['cv'][:, :, :1].expand(1, 384, 2, 128))
+    bad(cv=torch.zeros(1, 2, 384, 128, dtype=torch.bfloat16).transpose(1, 2))     # k and v in one layout
 
 
 def test_attention_rejects_bad_arguments():
@@ -87,6 +90,7 @@ def test_attention_rejects_bad_arguments():
     bad(scale=0.0)
     bad(scale=float('nan'))
     bad(out=a['q'][:4])
+    bad(out=a['q'][:1].expand(6, 4, 128))
     bad(TypeError, out=a['q'].half())
     bad(table=torch.zeros(5, 2, dtype=torch.int32), held=torch.zeros(5, dtype=torch.int32))
 
@@ -134,7 +138,8 @@ def test_append_abi_rejects():
                    dict(width=0), dict(pairs=65), dict(pairs=-1), dict(pairs=12, axis0=12, flags=0), dict(freqs=None),
                    dict(axes=0), dict(axes=4), dict(axis0=65), dict(axis0=40, axis1=40), dict(axes=2), dict(flags=4),
                    dict(k=None), dict(v=None), dict(ck=None), dict(cv=None), dict(table=None), dict(held=None),
-                   dict(q=None), dict(out=None), dict(k=4100), dict(kv_tok=260), dict(q_tok=-512), dict(k_head=4)):
+                   dict(q=None), dict(out=None), dict(k=4100), dict(kv_tok=260), dict(q_tok=-512), dict(k_head=4),
+                   dict(kv_tok=64)):
         assert append_call(**{'tokens': 2, **change}) == INVALID, change
 
 
