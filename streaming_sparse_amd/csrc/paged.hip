@@ -332,6 +332,13 @@ __device__ __forceinline__ void loads_left() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// All waves of a workgroup, their LDS reads and writes done.
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");      // nothing behind it is read ahead of it
+}
+
 // Writes what a lane holds of a row: 16 groups of 4 dims (8 c + 4 hh of row
 // rho = j.rho0 + 32 blk + lane % 32), the maximum M and the sum l; to the row's
 // state, or to out and lse.
@@ -781,8 +788,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     else
       loads_left<0>();
     clear_rows(begin, rows_ahead[0]);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
+    meet();
     S = f32x16{};
     if (alive) {
 #pragma unroll
@@ -798,9 +804,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
       f32x16 S1;
       if (alive) half_step(slot_c, std::integral_constant<int, 0>{}, S, S1, u, rows_ahead[0]);
       rows_ahead[3] = issue(u + 3);
-      if (alive) {
-        half_step(slot_c, std::integral_constant<int, 1>{}, S1, S, u + 1, rows_ahead[1]);
-      }
+      if (alive) half_step(slot_c, std::integral_constant<int, 1>{}, S1, S, u + 1, rows_ahead[1]);
       // next: K of unit u + 2 and V of unit u + 1; each unit is 2 loads of K,
       // then 2 of V
       if (u + 3 < end)
@@ -811,8 +815,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
       rows_ahead[1] = rows_ahead[2];
       rows_ahead[2] = rows_ahead[3];
       if (u + 1 < end) clear_rows(u + 1, rows_ahead[0]);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
+      meet();
       return ++u < end;
     };
     while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{}) &&
@@ -1002,12 +1005,33 @@ struct Plan {
   long long bytes(int kv_heads) const { return 4ll * kState * states(kv_heads); }
 };
 
-// Estimates, in us, that the pieces are chosen by: a workgroup's start and end,
-// a page of a tile, a state written and read again.
-constexpr double kStart = 7.0, kJoinStart = 3.0, kSoloPage = 5.0, kNarrowPage = 0.75;
-double wide_page(double rows) { return 1.0 + 0.9 * std::min(1.0, rows / kWide); }
+// Estimates, in us, that the pieces are chosen by, from captured calls (224, 96 and
+// 32 workgroups, 17 and 65 pages each): a workgroup's start and end and a page of its
+// tile, a state written and read again, pages from memory.  A wide tile's page
+// takes 0.93 to 0.98 us with up to 128 rows (a wave on each SIMD), 1.35 with 192,
+// with 256 1.62 where all CUs work and 1.32 where few do (the clock falls under the
+// matrix pipe's load); a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A
+// page that no other tile reads takes 1.1 and 1.2 at least, which is what one
+// workgroup draws from memory.
+constexpr double kJoinStart = 3.0, kSoloPage = 5.0;
+double start_time(int T, double rows) { return T == kWide ? 6.0 + 5.0 * rows / kWide : 7.0; }
+double tile_page(int T, double rows, double active, double cus, double unshared) {
+  const double busy = active / cus;
+  double page;
+  if (T == kNarrow) {
+    page = 0.47 + 0.25 * std::min(1.0, std::max(0.0, busy - 1.0));
+  } else {
+    const double second = std::max(0.0, std::ceil(rows / 32) - 4) / 4;     // SIMDs with two waves
+    page = second > 0 ? 1.3 + 0.3 * std::min(1.0, busy) * second * second : 0.95;
+  }
+  return page + unshared * std::max(0.0, (T == kNarrow ? 1.2 : 1.1) - page);
+}
 double state_time(double rows) { return rows * 2 * (4.0 * kState / 32) / 4.5e6; }
-double page_time(double pages) { return pages * 32768 / 5.2e6; }
+// Two workgroups on a CU draw less together (8 heads behind 30000 rows: 32 pieces
+// each 31.9 us, 64 38.9).
+double page_time(double pages, double busy = 1.0) {
+  return pages * 32768 / 5.2e6 * (1.0 + 0.2 * std::max(0.0, busy - 1.0));
+}
 
 constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64, 96, 128, 192, 256};
 
@@ -1063,19 +1087,21 @@ double plan_apart(const Sizes& z, Plan* plan) {
   plan->own_whole = 0;
   plan->longest_first = false;
   const double tiles = (double)z.kv_heads * plan->prefix_tiles, own_tiles = (double)z.kv_heads * plan->own_tiles;
-  const double page = wide ? wide_page((double)rows / plan->prefix_tiles) : kNarrowPage;
+  const double live = (double)rows / plan->prefix_tiles;
   const double floor_time = page_time(z.kv_heads * (prefix_pages + 0.6 * z.batch * z.table_pages));
   double least = 1e30;
   for (int c : kCuts) {
     if (c > 1 && 2 * c > prefix_pages) break;
     int cut;
     const int pieces = cut_in(prefix_pages, c, &cut);
-    const double t = kStart + cut * page;
+    const double t = start_time(T, live) + cut * tile_page(T, std::min<double>(rows, T),
+                                                           std::min(tiles * pieces, (double)slots), z.cus,
+                                                           plan->prefix_tiles == 1 ? 1.0 : 0.0);
     for (int d : kCuts) {
       if (d > 16 || (d > 1 && 2 * d > z.table_pages)) break;
       int own_cut;
       const int own = cut_in(z.table_pages, d, &own_cut);
-      const double u = kStart + own_cut * kSoloPage;
+      const double u = start_time(kNarrow, kNarrow) + own_cut * kSoloPage;
       const double cost = std::max(floor_time, makespan(tiles * pieces, t, own_tiles * own / waves, u, slots)) +
                           state_time((double)z.kv_heads * rows * (pieces + own)) + kJoinStart;
       if (cost < least) {
@@ -1108,8 +1134,14 @@ double plan_joint(const Sizes& z, Plan* plan) {
   const long long own_tiles = (long long)z.kv_heads * plan->own_tiles;
   const long long whole = wide && !plan->longest_first ? own_tiles / z.cus * z.cus : 0;
   const double tiles = (double)(own_tiles - whole);
-  const double live = per_seq / std::ceil(per_seq / T);     // rows of a tile that there are
-  const double page = wide ? wide_page(live) : kNarrowPage;
+  const double full = std::min<double>(per_seq, T);         // rows of the fullest tile
+  const double live = per_seq / std::ceil(per_seq / T);     // and of the mean one
+  const double start = start_time(T, live);
+  // the part of all lists' pages that come from memory, and of a list that no other
+  // tile reads
+  const double read = std::min(1.0, z.kv_heads * (z.prefix_pages() + (double)z.batch * z.table_pages) /
+                                        ((double)own_tiles * units));
+  const double unshared = per_seq > T ? 0.0 : z.batch == 1 ? 1.0 : (double)z.table_pages / units;
   double least = tiles > 0 ? 1e30 : 0.0;
   plan->own_pieces = 1;
   plan->own_cut = units;
@@ -1117,15 +1149,19 @@ double plan_joint(const Sizes& z, Plan* plan) {
     if (tiles == 0 || (c > 1 && 2 * c > units)) break;
     int cut;
     const int pieces = cut_in(units, c, &cut);
-    const double longest = kStart + cut * page;
     double time, states = 0.0;
     if (plan->longest_first) {
       const double mean = units - 0.5 * spread, each = std::max(1.0, mean / cut + (c > 1 ? 0.5 : 0.0));
+      const double page = tile_page(T, full, std::min(tiles * each, (double)slots), z.cus, unshared);
+      const double longest = start + cut * page;
       time = tiles * each <= slots ? longest
-                                   : std::max(longest, tiles * (each * kStart + mean * page) / slots + 0.5 * longest);
+                                   : std::max(longest, tiles * (each * start + mean * page) / slots + 0.5 * longest);
       states = c > 1 ? tiles * each : 0.0;
     } else {
-      time = std::ceil(tiles * pieces / slots) * std::max(longest, page_time(std::min(tiles * pieces, (double)slots) * cut));
+      const double active = std::min(tiles * pieces, (double)slots);
+      time = std::ceil(tiles * pieces / slots) *
+             (start + std::max(cut * tile_page(T, full, active, z.cus, unshared),
+                               page_time(read * active * cut, active / z.cus)));
       states = pieces > 1 ? tiles * pieces : 0.0;
     }
     const double cost = time + (states > 0 ? state_time(states * live) + kJoinStart : 0.0);
@@ -1136,7 +1172,7 @@ double plan_joint(const Sizes& z, Plan* plan) {
     }
   }
   plan->own_whole = (int)(plan->own_pieces == 1 ? own_tiles : whole);
-  return least + (double)(whole / z.cus) * (kStart + units * page);
+  return least + (double)(whole / z.cus) * (start + units * tile_page(T, full, slots, z.cus, unshared));
 }
 
 // The plan of a call's sizes (z.cus is filled in).  A thread keeps its last one:

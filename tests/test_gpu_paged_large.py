@@ -22,7 +22,8 @@ BF16, FP16 = torch.bfloat16, torch.float16
 
 CASES = [
     # batch, new tokens, equal, held, heads, K/V heads, prefix, causal, dtype
-    pytest.param(9, 1, True, 200, 3, 1, 5000, True, BF16, id='apart_narrow'),
+    pytest.param(8, 1, True, 200, 8, 8, 9000, True, BF16, id='apart_narrow'),
+    pytest.param(9, 1, True, 200, 3, 1, 5000, True, BF16, id='joint_narrow_pieces'),
     pytest.param(90, 1, True, 700, 6, 2, 20000, True, BF16, id='apart_wide_many_pieces'),
     pytest.param(30, 7, True, 90, 14, 2, 700, True, FP16, id='apart_wide_few_pieces'),
     pytest.param(12, 41, False, 300, 8, 8, 1500, True, BF16, id='apart_ragged'),
