@@ -40,7 +40,7 @@ extern "C" {
  * axis 2.  Angles are formed in float64; each result is rounded once.
  *
  * q [tokens, heads, 128] goes to q_out (which may be q itself); heads = 0: no
- * queries.  k and v must not overlap the cache rows written. */
+ * queries.  k and v must not overlap the cache rows written.  tokens < 2^26. */
 int ssa_paged_append(const void* q, long long q_token_stride, long long q_head_stride, void* q_out,
                      long long out_token_stride, long long out_head_stride, const void* k, long long k_token_stride,
                      long long k_head_stride, const void* v, long long v_token_stride, long long v_head_stride,
@@ -62,7 +62,8 @@ int ssa_paged_append(const void* q, long long q_token_stride, long long q_head_s
  * Rows of out and lse from starts[batch] on are left as they were.  Pages
  * outside [0, pages) count as absent: none of their rows is seen.  Values in
  * rows of a page that no query sees (behind a sequence's or the prefix's end)
- * may be anything, NaN included.
+ * may be anything, NaN included; one that some query of the call sees must be
+ * finite for the others to come out finite.  out may be q itself.
  *
  * workspace: 16-byte aligned, at least ssa_paged_attention_workspace_bytes of
  * the same sizes, any contents; calls that share one must not overlap. */
@@ -74,7 +75,7 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
                         float scale, int flags, void* workspace, long long workspace_bytes, hipStream_t stream);
 
 /* Bytes of that workspace (0: none needed), from sizes alone; -1 for sizes the
- * call rejects.  ragged: whether the call gives starts; causal: whether it is. */
+ * call rejects (tokens * heads >= 2^30, or more work than a grid holds).  ragged: whether the call gives starts; causal: whether it is. */
 long long ssa_paged_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int prefix_tokens,
                                               int table_pages, int ragged, int causal);
 

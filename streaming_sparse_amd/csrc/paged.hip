@@ -1003,6 +1003,24 @@ struct Plan {
     return own_pieces > 1 ? split_tiles(kv_heads) * own_pieces * (rows / 32) : 0;
   }
   long long bytes(int kv_heads) const { return 4ll * kState * states(kv_heads); }
+  // workgroups of the launches, and whether a grid holds them (2^32 threads)
+  int waves() const { return rows == kWide ? kWideWaves : kNarrowWaves; }
+  long long prefix_items(int kv_heads) const { return 1ll * kv_heads * prefix_tiles * prefix_pieces; }
+  long long own_items(int kv_heads) const { return own_whole + split_tiles(kv_heads) * own_pieces; }
+  long long items(int kv_heads) const {
+    const long long own = own_items(kv_heads);
+    return prefix_items(kv_heads) + (apart() ? (own + waves() - 1) / waves() : own);   // apart: a wave each
+  }
+  bool many() const { return prefix_pieces + own_pieces > kJoin; }
+  long long joins(int kv_heads) const {
+    const long long blocks =
+        apart() ? 1ll * kv_heads * row_tiles : own_pieces > 1 ? split_tiles(kv_heads) * (rows / 32) : 0;
+    return (many() ? 8 : 4) * blocks;
+  }
+  bool fits(int kv_heads) const {
+    return own_items(kv_heads) <= 0x7fffffffll && items(kv_heads) * 64 * waves() < (1ll << 32) &&
+           joins(kv_heads) * 64 * kJoinWaves < (1ll << 32);
+  }
 };
 
 // Estimates, in us, that the pieces are chosen by, from captured calls (224, 96 and
@@ -1201,7 +1219,8 @@ long long ssa_paged_attention_workspace_bytes(int tokens, int batch, int heads, 
   Plan plan;
   if (!sizes_fit(tokens, batch, heads, kv_heads, prefix_tokens, table_pages, ragged != 0) ||
       make_plan(Sizes{0, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, ragged != 0, causal != 0}, &plan) !=
-          (int)hipSuccess)
+          (int)hipSuccess ||
+      !plan.fits(kv_heads))
     return -1;
   return plan.bytes(kv_heads);
 }
@@ -1213,7 +1232,7 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
                         float* lse, int tokens, int batch, int heads, int kv_heads, int pages, int table_pages,
                         float scale, int flags, void* workspace, long long workspace_bytes, hipStream_t stream) {
   if (!sizes_fit(tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr) || pages <= 0 ||
-      (flags & ~3) || !(scale > 0.0f))
+      (flags & ~3) || !(scale > 0.0f && scale < INFINITY))
     return (int)hipErrorInvalidValue;
   if (!q || !cache_k || !cache_v || !table || !lengths || !out || (prefix_tokens > 0 && !prefix))
     return (int)hipErrorInvalidValue;
@@ -1227,6 +1246,7 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   const int e = make_plan(Sizes{0, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr,
                                 (flags & 2) != 0}, &plan);
   if (e != (int)hipSuccess) return e;
+  if (!plan.fits(kv_heads)) return (int)hipErrorInvalidValue;
   const long long need = plan.bytes(kv_heads);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return (int)hipErrorInvalidValue;
@@ -1268,18 +1288,10 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   p.own_cut = plan.own_cut;
   p.longest_first = plan.longest_first;
   p.apart = plan.apart();
-  const long long prefix_items = 1ll * kv_heads * plan.prefix_tiles * plan.prefix_pieces;
-  const bool wide = plan.rows == kWide;
-  long long own_items = plan.own_whole + plan.split_tiles(kv_heads) * plan.own_pieces;
-  if (own_items > 0x7fffffffll) return (int)hipErrorInvalidValue;
-  const int waves = wide ? kWideWaves : kNarrowWaves;
-  if (plan.apart()) own_items = (own_items + waves - 1) / waves;    // a wave each
-  const long long items = prefix_items + own_items;
-  const bool many = plan.prefix_pieces + plan.own_pieces > kJoin;
-  const long long joins = (many ? 8 : 4) * (plan.apart() ? 1ll * kv_heads * plan.row_tiles
-                                            : plan.own_pieces > 1 ? plan.split_tiles(kv_heads) * (plan.rows / 32) : 0);
-  if (items > 0x7fffffffll || joins > 0x7fffffffll) return (int)hipErrorInvalidValue;
-  p.prefix_items = (int)prefix_items;
+  p.prefix_items = (int)plan.prefix_items(kv_heads);
+  const long long items = plan.items(kv_heads), joins = plan.joins(kv_heads);
+  const int waves = plan.waves();
+  const bool wide = plan.rows == kWide, many = plan.many();
   const bool f16 = flags & 1;
   auto launch = [&](auto kernel, long long blocks, int threads) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, p);

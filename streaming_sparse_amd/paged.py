@@ -131,9 +131,9 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
     the first axis, and so on (axes: up to 3 counts that sum to R).  Angles
     are formed in float64.
 
-    q_out: where the rotated queries go (q itself is allowed); else a buffer
-    owned by `workspace` that the next call overwrites, or, without one, a new
-    tensor."""
+    q_out: where the rotated queries go (q itself is allowed; otherwise it must
+    not overlap what is read); else a buffer owned by `workspace` that the next
+    call overwrites, or, without one, a new tensor."""
     device, dtype, dev = k.device, k.dtype, k.get_device()
     code = _TYPES.get(dtype)
     if code is None:
@@ -188,7 +188,9 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
     return q_out
 
 
-_BYTES = {}     # workspace bytes by sizes and device
+# Workspace bytes by sizes and device, rounded up to a power of two: calls of many
+# sizes share a few buffers.
+_BYTES = {}
 
 
 def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, workspace, *, starts=None, causal=True,
@@ -211,7 +213,7 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     scale defaults to 128 ** -0.5.  Returns out [N, H, 128], or (out, lse)
     with want_lse, lse [N, H] float32 the log of the sum of exponentials:
     buffers owned by `workspace` and overwritten by the next call, or `out` as
-    given.
+    given (q itself is allowed; otherwise it must not overlap what is read).
 
     Arithmetic: scores, maxima, sums and the joins of pieces are float32.  A
     probability meets V in 16 bits: in two parts (hi + lo) where a tile is
@@ -260,8 +262,8 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
 
 
 def _workspace_bytes(key, device):
-    """The workspace that a call of these sizes needs, asked of the library once
-    per sizes and device."""
+    """The workspace of a call of these sizes, asked of the library once per sizes
+    and device."""
     tokens, batch, heads, kv_heads, prefix_tokens, width, equal, causal, dev = key
     if dev < 0:
         raise RuntimeError("the tensors must be on a GPU")
@@ -270,6 +272,8 @@ def _workspace_bytes(key, device):
                                                               int(not equal), int(bool(causal)))
     if need < 0:
         raise ValueError("paged.attention: sizes out of range")
+    if need:
+        need = 1 << (need - 1).bit_length()
     if len(_BYTES) >= 4096:
         _BYTES.clear()
     _BYTES[key] = need

@@ -19,7 +19,7 @@ import pytest
 import torch
 
 from oracle import paged as oracle
-from streaming_sparse_amd import paged
+from streaming_sparse_amd import _lib, paged
 from streaming_sparse_amd.attention import Workspace
 
 pytestmark = pytest.mark.gpu
@@ -263,6 +263,24 @@ def test_attention_two_streams_at_once(device):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
+def test_attention_workspace_of_many_sizes(device):
+    """Calls of many sizes, as a server makes them, share a few buffers for their
+    pieces."""
+    ws = Workspace()
+    for n in range(1, 25):
+        c = Case(device, [1] * n, [40] * n, 4, 2, 600)
+        c.check(*c.attend(ws=ws))
+    sizes = [key[1][0] for key in ws.entries if key[0] == 'paged_part']
+    assert sizes and len(sizes) <= 8 and all(x & (x - 1) == 0 for x in sizes)
+
+
+def test_attention_sizes_that_no_grid_holds(device):
+    """2^25 tiles of 256 threads are refused before anything is launched."""
+    size = _lib.lib().ssa_paged_attention_workspace_bytes
+    assert size(1 << 20, 1 << 20, 32, 32, 0, 1, 0, 1) == -1
+    assert size(1 << 18, 1 << 18, 32, 32, 0, 1, 0, 1) >= 0
 
 
 def append_case(device, c, k, v, **more):

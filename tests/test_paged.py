@@ -139,7 +139,7 @@ def test_append_abi_rejects():
                    dict(axes=0), dict(axes=4), dict(axis0=65), dict(axis0=40, axis1=40), dict(axes=2), dict(flags=4),
                    dict(k=None), dict(v=None), dict(ck=None), dict(cv=None), dict(table=None), dict(held=None),
                    dict(q=None), dict(out=None), dict(k=4100), dict(kv_tok=260), dict(q_tok=-512), dict(k_head=4),
-                   dict(kv_tok=64)):
+                   dict(kv_tok=64), dict(tokens=1 << 26)):
         assert append_call(**{'tokens': 2, **change}) == INVALID, change
 
 
@@ -155,9 +155,9 @@ def attention_call(**change):
 def test_attention_abi_rejects():
     for change in (dict(tokens=0), dict(tokens=3), dict(batch=0), dict(heads=3), dict(heads=0), dict(kv_heads=0),
                    dict(pages=0), dict(width=0), dict(prefix_tokens=-1), dict(prefix=None), dict(scale=0.0),
-                   dict(scale=float('nan')), dict(flags=4), dict(q=None), dict(ck=None), dict(cv=None), dict(table=None),
-                   dict(lengths=None), dict(out=None), dict(q=4098), dict(lse=4098), dict(kv_tok=64), dict(kv_tok=260),
-                   dict(o_tok=-8), dict(tokens=1 << 30, batch=1 << 10), dict(width=1 << 26), dict(kv_tok=1 << 24)):
+                   dict(scale=float('nan')), dict(scale=float('inf')), dict(flags=4), dict(q=None), dict(ck=None),
+                   dict(cv=None), dict(table=None), dict(lengths=None), dict(out=None), dict(q=4098), dict(lse=4098),
+                   dict(kv_tok=64), dict(kv_tok=260), dict(o_tok=-8), dict(tokens=1 << 30, batch=1 << 10), dict(width=1 << 26), dict(kv_tok=1 << 24)):
         assert attention_call(**change) == INVALID, change
     size = _lib.lib().ssa_paged_attention_workspace_bytes
     assert size(3, 2, 4, 2, 0, 1, 0, 1) == -1 and size(2, 2, 4, 3, 0, 1, 0, 1) == -1 and size(0, 1, 1, 1, 0, 1, 0, 1) == -1
