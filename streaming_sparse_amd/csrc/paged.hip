@@ -32,6 +32,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
 
 constexpr int kPage = 64;
 
@@ -332,6 +333,21 @@ __device__ __forceinline__ void loads_left() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// 16 bytes from each lane's own address into lds + 16 * lane; not counted by the
+// compiler, as dma_rows.
+__device__ __forceinline__ void dma_at(const void* from, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(lds) : "memory");
+}
+
+// Lane `from`'s pointer.
+template <typename T>
+__device__ __forceinline__ T* of_lane(T* p, int from) {
+  const uint64_t a = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_ds_bpermute(from << 2, (int)(uint32_t)a);
+  const uint32_t hi = __builtin_amdgcn_ds_bpermute(from << 2, (int)(uint32_t)(a >> 32));
+  return (T*)((uint64_t)hi << 32 | lo);
+}
+
 // All waves of a workgroup, their LDS reads and writes done.
 __device__ __forceinline__ void meet() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -339,41 +355,26 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");      // nothing behind it is read ahead of it
 }
 
-// Writes what a lane holds of a row: 16 groups of 4 dims (8 c + 4 hh of row
-// rho = j.rho0 + 32 blk + lane % 32), the maximum M and the sum l; to the row's
-// state, or to out and lse.
-template <bool F16, int T>
-__device__ __forceinline__ void finish_row(const PagedParams& p, const Job& j, const f32x16 (&O)[4], float M, float l,
-                                           int blk, int lane) {
+// Writes what a lane holds of a row to the row's state: 16 groups of 4 dims (8 c +
+// 4 hh of row rho = j.rho0 + 32 blk + lane % 32), the maximum M and the sum l.
+template <int T>
+__device__ __forceinline__ void write_state(const PagedParams& p, const Job& j, const f32x16 (&O)[4], float M, float l,
+                                            int blk, int lane) {
   const int rho = j.rho0 + 32 * blk + (lane & 31), hh = lane >> 5;
   if (rho >= j.rho1) return;
-  if (j.state >= 0) {
-    int col;
-    float* st = state_of<T>(p, j, rho, blk, &col);
-    // the sums of an empty state are not read
+  int col;
+  float* st = state_of<T>(p, j, rho, blk, &col);
+  // the sums of an empty state are not read
 #pragma unroll
-    for (int c = 0; c < 16 && j.begin < j.end; ++c) {
-      const f32x16& o = O[c >> 2];
-      const int i = 4 * (c & 3);
-      *reinterpret_cast<f32x4*>(st + ((2 * c + hh) * 32 + col) * 4) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
-    }
-    if (hh == 0) {
-      st[32 * kHeadDim + col] = M;
-      st[32 * kHeadDim + 32 + col] = l;
-    }
-    return;
-  }
-  const int token = rho / p.group, hq = j.h * p.group + rho % p.group;
-  const bool none = __float_as_uint(l) == 0u;
-  const float inv = none ? 0.0f : 1.0f / l;
-  uint16_t* op = p.out + (long long)token * p.o_tok + (long long)hq * p.o_head + 4 * hh;
-#pragma unroll
-  for (int c = 0; c < 16; ++c) {
-    const f32x16 o = O[c >> 2] * inv;
+  for (int c = 0; c < 16 && j.begin < j.end; ++c) {
+    const f32x16& o = O[c >> 2];
     const int i = 4 * (c & 3);
-    *reinterpret_cast<u32x2*>(op + 8 * c) = u32x2{pack2<F16>(o[i], o[i + 1]), pack2<F16>(o[i + 2], o[i + 3])};
+    *reinterpret_cast<f32x4*>(st + ((2 * c + hh) * 32 + col) * 4) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
   }
-  if (p.lse && hh == 0) p.lse[(long long)token * p.heads + hq] = lse_of(M, l);
+  if (hh == 0) {
+    st[32 * kHeadDim + col] = M;
+    st[32 * kHeadDim + 32 + col] = l;
+  }
 }
 
 // NW waves share a tile; NW = 1: a wave by itself.
@@ -514,7 +515,7 @@ __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, 
   const float l = half_sum(ls);
   const float mine = m == -INFINITY ? m : m - kLift<F16>;
   if constexpr (NW == 1) {
-    finish_row<F16, kNarrow>(p, j, O, mine, l, 0, e);
+    write_state<kNarrow>(p, j, O, mine, l, 0, e);      // beside prefix tiles, so never the last word
   } else {
     // the waves' states into one: every wave hands over m, l and its 32 x 128
     // sums, [dim tile][j][lane] of 4 floats, two dim tiles at a time (8 KB a wave;
@@ -623,14 +624,12 @@ template <bool F16>
 __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
   const int r = lane & 31, hh = lane >> 5;
   int limit;                                  // rows of its sequence that the lane's row sees
-  u32x4 qop[8];
+  const uint16_t* qp;
   {
     const int rho = min(j.rho0 + 32 * wave + r, j.rho1 - 1);
     const int token = rho / p.group, hq = j.h * p.group + rho % p.group;
     limit = p.causal ? j.length - j.n + (token - j.first_token) + 1 : j.length;
-    const uint16_t* qp = p.q + (long long)token * p.q_tok + (long long)hq * p.q_head + 8 * hh;
-#pragma unroll
-    for (int st = 0; st < 8; ++st) qop[st] = ldg16(qp + 16 * st);
+    qp = p.q + (long long)token * p.q_tok + (long long)hq * p.q_head;
   }
   // what every row of the wave sees of its sequence; a wave without rows only
   // loads
@@ -654,6 +653,22 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   const uint8_t* const vh = (const uint8_t*)(p.v + (long long)j.h * p.kv_head);
   PageList list(p, j, begin, lane);
   wait_loads();       // as in narrow_tile
+  // The query rows, and in the end the output's, go by way of the parts of slots 2
+  // and 3 that this wave itself loads (8 rows of each of the four 16 KB), so that
+  // memory sees whole rows and no wave waits for another.  Operands' own form, 32
+  // bytes of 32 rows an instruction, took 3.0 us of a tile's start and 3.8 of its
+  // end where all CUs begin and end together.  Chunk c of row x lies at c ^ (x &
+  // 15).
+  auto own_row = [&](int x) {
+    return ring + (2 + (x >> 4)) * kTile + ((x >> 3) & 1) * (kSlots * kTile) + wave * 2048 + (x & 7) * 256;
+  };
+  auto chunk_of = [](int x, int c) { return (c ^ (x & 15)) << 4; };
+#pragma unroll
+  for (int jj = 0; jj < 8; ++jj) {
+    const int x = 4 * jj + (lane >> 4);
+    dma_at((const uint8_t*)of_lane(qp, x) + chunk_of(x, lane & 15),
+           __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)own_row(4 * jj)));
+  }
   int rows_ahead[kSlots] = {0, 0, 0, 0};    // rows of units i .. i + 3
   auto issue = [&](int u) {
     if (u >= end) return 0;
@@ -665,8 +680,17 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     dma_rows<2>(vh + at, voff, l + kSlots * kTile);
     return x.rows;
   };
+  rows_ahead[0] = issue(begin);
+  rows_ahead[1] = issue(begin + 1);
+  if (begin + 2 <= end)
+    loads_left<8>();            // the query rows landed, two units behind them
+  else
+    loads_left<0>();
+  u32x4 qop[8];
 #pragma unroll
-  for (int u = 0; u < kSlots - 1; ++u) rows_ahead[u] = issue(begin + u);
+  for (int st = 0; st < 8; ++st) qop[st] = *(lds_u32x4*)(own_row(r) + chunk_of(r, 2 * st + hh));
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  rows_ahead[2] = issue(begin + 2);
 
   f32x16 O[4], S;
 #pragma unroll
@@ -826,7 +850,30 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   // the lane's row, formed anew so that no register holds it across the loop
   int e = lane;
   asm volatile("" : "+v"(e));
-  finish_row<F16, kWide>(p, j, O, m == -INFINITY ? m : m - kLift<F16>, half_sum(ls), wave, e);
+  const float M = m == -INFINITY ? m : m - kLift<F16>, l = half_sum(ls);
+  if (j.state >= 0) {
+    write_state<kWide>(p, j, O, M, l, wave, e);
+    return;
+  }
+  const int x = e & 31, he = e >> 5, rho = j.rho0 + 32 * wave + x;
+  const int token = rho / p.group, hq = j.h * p.group + rho % p.group;
+  uint16_t* const to = p.out + (long long)token * p.o_tok + (long long)hq * p.o_head;
+  const float inv = __float_as_uint(l) == 0u ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    const f32x16 o = O[c >> 2] * inv;
+    const int i = 4 * (c & 3);
+    *(lds_u32x2*)(own_row(x) + chunk_of(x, c) + 8 * he) =
+        u32x2{pack2<F16>(o[i], o[i + 1]), pack2<F16>(o[i + 2], o[i + 3])};
+  }
+#pragma unroll
+  for (int jj = 0; jj < 8; ++jj) {
+    const int y = 4 * jj + (e >> 4);
+    uint16_t* const at = of_lane(to, y);
+    const u32x4 w = *(lds_u32x4*)(own_row(y) + chunk_of(y, e & 15));
+    if (j.rho0 + 32 * wave + y < j.rho1) *reinterpret_cast<u32x4*>(at + 8 * (e & 15)) = w;
+  }
+  if (p.lse && he == 0 && rho < j.rho1) p.lse[(long long)token * p.heads + hq] = lse_of(M, l);
 }
 
 // APART: prefix tiles, then own tiles of 32 rows, eight to a workgroup, a wave
