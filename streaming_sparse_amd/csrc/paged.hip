@@ -55,6 +55,7 @@ struct PagedParams {
   int prefix_items, prefix_tiles, prefix_pieces, prefix_cut, own_tiles, own_whole, own_pieces, own_cut, apart,
       longest_first;
   int row_tiles;      // 32-row tiles of a K/V head's rows, where the prefix is apart
+  int own_waves;      // and the waves of a workgroup that take own items then
 };
 
 // A piece's state of 32 rows: O [dim / 4][row] of 4 floats, m [32], l [32].  Where
@@ -588,6 +589,22 @@ __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, 
   }
 }
 
+// Where the prefix is apart: the own items of workgroup `group` of `groups`, a wave
+// each, one after the other.  Waves that begin and end at different times keep the
+// CU's loads on their way, where a workgroup for every eight items leaves it idle
+// between them.
+template <bool F16>
+__device__ __forceinline__ void own_items(const PagedParams& p, int group, int groups, lds_u8* ring, int lane,
+                                          int wave) {
+  if (wave >= p.own_waves) return;
+  const int all = p.kv_heads * p.own_tiles * p.own_pieces;
+  Job j;
+  for (long long own = group * p.own_waves + wave; own < all; own += (long long)groups * p.own_waves) {
+    if (own_job<kNarrow>(p, (int)own, lane, j)) narrow_tile<F16, 1>(p, j, ring, lane, wave);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // its rows are read before the next ones come
+  }
+}
+
 // APART: prefix tiles, then own tiles, a wave each.
 template <bool F16, bool APART>
 __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParams p) {
@@ -600,9 +617,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
     if (b < first) {
       if (prefix_job<kNarrow>(p, item, j)) narrow_tile<F16, kNarrowWaves>(p, j, (lds_u8*)ring, lane, wave);
     } else {
-      const int own = item * kNarrowWaves + wave;
-      if (own < p.kv_heads * p.own_tiles * p.own_pieces && own_job<kNarrow>(p, own, lane, j))
-        narrow_tile<F16, 1>(p, j, (lds_u8*)ring, lane, wave);
+      own_items<F16>(p, item, gridDim.x - first, (lds_u8*)ring, lane, wave);
     }
   } else {
     if (own_job<kNarrow>(p, item, lane, j)) narrow_tile<F16, kNarrowWaves>(p, j, (lds_u8*)ring, lane, wave);
@@ -893,9 +908,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p)
     if (b < first) {
       if (prefix_job<kWide>(p, item, j)) wide_tile<F16>(p, j, (lds_u8*)ring, lane, wave);
     } else {
-      const int own = item * kWideWaves + wave;
-      if (own < p.kv_heads * p.own_tiles * p.own_pieces && own_job<kNarrow>(p, own, lane, j))
-        narrow_tile<F16, 1>(p, j, (lds_u8*)ring, lane, wave);
+      own_items<F16>(p, item, gridDim.x - first, (lds_u8*)ring, lane, wave);
     }
   } else {
     if (own_job<kWide>(p, b < first ? item : first + item, lane, j))
@@ -1042,6 +1055,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedParams p) {
 // (wide); own tiles beside prefix tiles are narrow.
 struct Plan {
   int rows, row_tiles, prefix_tiles, prefix_pieces, prefix_cut, own_tiles, own_whole, own_pieces, own_cut;
+  int own_groups, own_waves;     // apart: workgroups of own items, and their waves that take some
   bool longest_first;
   bool apart() const { return prefix_tiles > 0; }
   long long split_tiles(int kv_heads) const { return (long long)kv_heads * own_tiles - own_whole; }
@@ -1055,8 +1069,7 @@ struct Plan {
   long long prefix_items(int kv_heads) const { return 1ll * kv_heads * prefix_tiles * prefix_pieces; }
   long long own_items(int kv_heads) const { return own_whole + split_tiles(kv_heads) * own_pieces; }
   long long items(int kv_heads) const {
-    const long long own = own_items(kv_heads);
-    return prefix_items(kv_heads) + (apart() ? (own + waves() - 1) / waves() : own);   // apart: a wave each
+    return prefix_items(kv_heads) + (apart() ? own_groups : own_items(kv_heads));
   }
   bool many() const { return prefix_pieces + own_pieces > kJoin; }
   long long joins(int kv_heads) const {
@@ -1078,7 +1091,7 @@ struct Plan {
 // matrix pipe's load); a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A
 // page that no other tile reads takes 1.1 and 1.2 at least, which is what one
 // workgroup draws from memory.
-constexpr double kJoinStart = 3.0, kSoloPage = 5.0;
+constexpr double kJoinStart = 3.0, kSoloPage = 0.85, kSoloLatency = 3.5, kSoloStart = 3.0, kSoloItem = 5.0;
 double start_time(int T, double rows) { return T == kWide ? 6.0 + 5.0 * rows / kWide : 7.0; }
 double tile_page(int T, double rows, double active, double cus, double unshared) {
   const double busy = active / cus;
@@ -1099,16 +1112,6 @@ double page_time(double pages, double busy = 1.0) {
 }
 
 constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64, 96, 128, 192, 256};
-
-// When n workgroups of the time t each, and then m of the time u, are done on
-// `slots` places.
-double makespan(double n, double t, double m, double u, double slots) {
-  const double rounds = std::ceil(n / slots), done = rounds * t;
-  const double left = rounds * slots - n;                     // places that the last round leaves
-  const double after = done + std::ceil(std::max(0.0, m - left * std::floor(t / u)) / slots) * u;
-  const double beside = left > 0 ? done - t + std::ceil(m / left) * u : after;
-  return std::max(done, std::min(after, beside));
-}
 
 bool sizes_fit(int tokens, int batch, int heads, int kv_heads, int prefix_tokens, int table_pages, bool ragged) {
   return tokens > 0 && batch > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && prefix_tokens >= 0 &&
@@ -1143,17 +1146,41 @@ struct Sizes {
 double plan_apart(const Sizes& z, Plan* plan) {
   const long long rows = z.rows();
   const int T = rows <= kNarrow ? kNarrow : kWide, prefix_pages = z.prefix_pages();
-  const bool wide = T == kWide;
-  const int slots = wide ? z.cus : 2 * z.cus, waves = wide ? kWideWaves : kNarrowWaves;
+  const int slots = z.cus;
   plan->rows = T;
   plan->row_tiles = (int)((rows + 31) / 32);
   plan->prefix_tiles = (int)((rows + T - 1) / T);
   plan->own_tiles = z.seq_tiles(kNarrow);
   plan->own_whole = 0;
-  plan->longest_first = false;
+  plan->longest_first = true;
   const double tiles = (double)z.kv_heads * plan->prefix_tiles, own_tiles = (double)z.kv_heads * plan->own_tiles;
   const double live = (double)rows / plan->prefix_tiles;
   const double floor_time = page_time(z.kv_heads * (prefix_pages + 0.6 * z.batch * z.table_pages));
+  // pages of a sequence's mean list
+  const double spread = z.causal ? (double)(z.tokens / z.batch) / kPage : 0.0;
+  const double mean = std::max(1.0, z.table_pages - 0.5 * spread);
+  // n own items over at most *g workgroups, of which *w waves take some: as many as
+  // give every item a wave, or a power of two, with which the rows of the heads, that
+  // lie side by side, are read together
+  auto own_time = [&](double n, int cut, double* g, int* w) {
+    const double places = *g;
+    const int exact = (int)std::min<double>(plan->waves(), std::ceil(n / places));
+    double least = 1e30;
+    for (int x = 1; x <= plan->waves(); ++x) {
+      const bool even = !(x & (x - 1));
+      if (!even && x != exact) continue;
+      const double groups = std::min(places, std::ceil(n / x));
+      const double page = std::max({kSoloLatency, kSoloPage * x * (even ? 1.0 : 1.15), page_time(0.7 * groups * x)});
+      const double time =
+          kSoloStart + std::ceil(n / (groups * x)) * (kSoloItem + page * std::min<double>(cut, mean));
+      if (time < least) {
+        least = time;
+        *g = groups;
+        *w = x;
+      }
+    }
+    return least;
+  };
   double least = 1e30;
   for (int c : kCuts) {
     if (c > 1 && 2 * c > prefix_pages) break;
@@ -1162,19 +1189,36 @@ double plan_apart(const Sizes& z, Plan* plan) {
     const double t = start_time(T, live) + cut * tile_page(T, std::min<double>(rows, T),
                                                            std::min(tiles * pieces, (double)slots), z.cus,
                                                            plan->prefix_tiles == 1 ? 1.0 : 0.0);
+    const double rounds = std::ceil(tiles * pieces / slots), left = rounds * slots - tiles * pieces;
     for (int d : kCuts) {
       if (d > 16 || (d > 1 && 2 * d > z.table_pages)) break;
       int own_cut;
       const int own = cut_in(z.table_pages, d, &own_cut);
-      const double u = start_time(kNarrow, kNarrow) + own_cut * kSoloPage;
-      const double cost = std::max(floor_time, makespan(tiles * pieces, t, own_tiles * own / waves, u, slots)) +
-                          state_time((double)z.kv_heads * rows * (pieces + own)) + kJoinStart;
+      const double n = own_tiles * own;
+      // on the places that the last round of the prefix leaves, or behind it too
+      double g = slots;
+      int w;
+      double time = rounds * t + own_time(n, own_cut, &g, &w);
+      if (left > 0) {
+        double beside = left;
+        int v;
+        const double u = std::max(rounds * t, (rounds - 1) * t + own_time(n, own_cut, &beside, &v));
+        if (u < time) {
+          g = beside;
+          w = v;
+          time = u;
+        }
+      }
+      const double cost =
+          std::max(floor_time, time) + state_time((double)z.kv_heads * rows * (pieces + own)) + kJoinStart;
       if (cost < least) {
         least = cost;
         plan->prefix_pieces = pieces;
         plan->prefix_cut = cut;
         plan->own_pieces = own;
         plan->own_cut = own_cut;
+        plan->own_groups = (int)g;
+        plan->own_waves = w;
       }
     }
   }
@@ -1192,6 +1236,7 @@ double plan_joint(const Sizes& z, Plan* plan) {
   const int slots = wide ? z.cus : 2 * z.cus;
   plan->rows = T;
   plan->row_tiles = plan->prefix_tiles = plan->prefix_pieces = plan->prefix_cut = 0;
+  plan->own_groups = plan->own_waves = 0;
   plan->own_tiles = z.seq_tiles(T);
   // pages that the first tile of a sequence sees fewer of than the last
   const double spread = z.causal ? (double)(z.tokens / z.batch) / kPage : 0.0;
@@ -1326,6 +1371,7 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   p.causal = (flags & 2) != 0;
   p.scale_log2 = scale * kLog2e;
   p.row_tiles = plan.row_tiles;
+  p.own_waves = plan.own_waves;
   p.prefix_tiles = plan.prefix_tiles;
   p.prefix_pieces = plan.prefix_pieces;
   p.prefix_cut = plan.prefix_cut;

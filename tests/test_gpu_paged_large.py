@@ -27,6 +27,8 @@ CASES = [
     pytest.param(90, 1, True, 700, 6, 2, 20000, True, BF16, id='apart_wide_many_pieces'),
     pytest.param(30, 7, True, 90, 14, 2, 700, True, FP16, id='apart_wide_few_pieces'),
     pytest.param(12, 41, False, 300, 8, 8, 1500, True, BF16, id='apart_ragged'),
+    pytest.param(300, 1, True, 130, 16, 8, 700, True, BF16, id='apart_items_in_turn'),
+    pytest.param(200, 3, False, 500, 12, 12, 300, False, FP16, id='apart_ragged_items_in_turn'),
     pytest.param(1, 1, True, 30, 8, 2, 30000, True, FP16, id='joint_narrow_many_pieces'),
     pytest.param(40, 3, True, 400, 12, 12, 0, True, BF16, id='joint_narrow_whole'),
     pytest.param(1, 200, True, 50, 8, 2, 30000, True, BF16, id='joint_wide_many_pieces'),
