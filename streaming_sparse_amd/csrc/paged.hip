@@ -325,7 +325,8 @@ struct PageList {
 // its V as soon as V is read, and eight waves of a CU wait at different times, so
 // that something is always on its way.  The matrix pipe has time to spare:
 // probabilities meet V in two parts (hi + lo), so that no rounding of theirs
-// shows in the output.
+// shows in the output.  One token of 32 heads on 8 K/V heads behind 60000 rows:
+// 52.8 us, 4.7 TB/s (a large copy 5.1).
 constexpr int kNarrow = 32, kNarrowWaves = 4;
 constexpr int kHalf = 32 * 256;      // 32 rows of K or V
 
@@ -630,7 +631,16 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
 // the other's exponentials; each holds 32 rows with their sums in registers and
 // walks every key, and all share the pages.  S^T = K Q^T and O^T += V^T P^T on
 // 32 x 32 x 16 products: a lane holds one query, its softmax needs no other lane
-// but l ^ 32.
+// but l ^ 32.  A probability meets V rounded once: the second part would be half
+// as many products again, and the outputs are off by 1.4 times the rounding of
+// probabilities that are normalised first.
+// 4 sequences of 4608 tokens, 12 heads, behind 23040 rows: 2641 us, 1.19 PFLOP/s
+// (an 8192^3 library product 1.40), the matrix pipe busy 62% of the time and the
+// vector pipe 53 at the 1.8 GHz that the chip holds under this load.  Waves of 64
+// rows, one on a SIMD, read half as much LDS and took 2948 us where these took 2711;
+// from there the slots at fixed offsets, the raised priority and the loads between
+// the half pages.  The sums as dot products of the rounded pairs, half as many
+// instructions: 2703 us.
 constexpr int kWide = 256, kWideWaves = 8, kSlots = 4;
 constexpr int kTile = 64 * 256;      // a page's K or V rows
 
@@ -972,11 +982,12 @@ __device__ __forceinline__ Gathered<N> gather(const float* st, long long step, i
   return got;
 }
 
-// Joins the pieces' states of 32 rows of a K/V head: block (h, rows 32 T .., group)
+// Joins the pieces' states of 32 rows of a K/V head, 528 bytes a row and piece: block (h, rows 32 T .., group)
 // where the prefix is apart (T_ROWS 0), else (split tile of T_ROWS rows, block of
 // 32, group).  Bound by the latency of its loads.  Few pieces: a group is 32 dims, a
 // wave gathers 8 of them over all pieces.  MANY: a group is 16 dims, which the
-// four waves gather over a quarter of the pieces each; their sums meet in LDS.
+// four waves gather over a quarter of the pieces each; their sums meet in LDS (32
+// pieces, 8 rows: 3.7 us).
 template <bool F16, int T_ROWS, bool MANY>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedParams p) {
   constexpr int kGroups = MANY ? 8 : 4;
@@ -1090,7 +1101,9 @@ struct Plan {
 // with 256 1.62 where all CUs work and 1.32 where few do (the clock falls under the
 // matrix pipe's load); a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A
 // page that no other tile reads takes 1.1 and 1.2 at least, which is what one
-// workgroup draws from memory.
+// workgroup draws from memory.  Waves by themselves: a CU draws a page in 0.85 us (8
+// of them one each in 6.8), a wave one in 3.5, and an item begins and ends in 5.
+// Tables are taken to be 0.6 to 0.7 full, which only shifts the choice.
 constexpr double kJoinStart = 3.0, kSoloPage = 0.85, kSoloLatency = 3.5, kSoloStart = 3.0, kSoloItem = 5.0;
 double start_time(int T, double rows) { return T == kWide ? 6.0 + 5.0 * rows / kWide : 7.0; }
 double tile_page(int T, double rows, double active, double cus, double unshared) {
@@ -1142,7 +1155,13 @@ struct Sizes {
 };
 
 // The prefix apart: all rows together over the prefix, each sequence over its own
-// pages.  Returns the estimated time.
+// pages.  Returns the estimated time.  Against one list, us: 64 x 1 token, 32 heads on
+// 8, behind 16384: 48 and 228; 16 x 1 behind 131001: 118 and 1089; 24 x 5, 28 on 4,
+// behind 5003: 27 and 54; where sequences fill tiles, 8 x 1536 behind 4608, 579 and
+// 422.  The own lists' first pieces come first, then the second ones, on the CUs the
+// prefix leaves (64 x 1 behind 2048, up to 2000 own rows: 75, list by list 85), as
+// many workgroups as there are places, each wave several items (128 x 1 behind 4096,
+// up to 1000: 80, with a workgroup for every eight items 87).
 double plan_apart(const Sizes& z, Plan* plan) {
   const long long rows = z.rows();
   const int T = rows <= kNarrow ? kNarrow : kWide, prefix_pages = z.prefix_pages();
@@ -1226,9 +1245,13 @@ double plan_apart(const Sizes& z, Plan* plan) {
 }
 
 // Every tile over prefix and own pages.  Where their lists are alike and there
-// are more wide tiles than CUs, only those behind the last full round are cut;
-// where a causal sequence's first tiles have much shorter lists than its last,
-// every list is cut at the same length.
+// are more wide tiles than CUs, only those behind the last full round are cut
+// (8 x 1536 tokens, 12 heads, behind 4608: 422 us, 494 uncut); where a causal
+// sequence's first tiles have much shorter lists than its last, every list is cut
+// at the same length and the longest come first (2717 tokens, 12 heads: 58 us, 76
+// uncut, 76 in their order; 9 x 2786, 4 heads: 96, 127 in their order).  Sequences
+// of up to 32 rows a K/V head take narrow tiles (40 x 3 tokens: 16.3 us, 22.7 with
+// wide ones).
 double plan_joint(const Sizes& z, Plan* plan) {
   const double per_seq = (double)z.rows() / z.batch;
   const int T = per_seq <= kNarrow ? kNarrow : kWide, units = z.table_pages + z.prefix_pages();
