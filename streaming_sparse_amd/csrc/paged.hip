@@ -155,8 +155,8 @@ struct Job {
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
 // Sequence and tile of the idx-th tile of T rows, sequence by sequence (each
-// sequence's last tile may be short); b = -1 behind the last.  One pass per 64
-// sequences: every lane counts one sequence's tiles, a wave scan sums them.
+// sequence's last tile may be short); b = -1 behind the last.  One pass per 256
+// sequences: every lane counts four sequences' tiles, a wave scan sums them.
 // `last_first`: the last tile of each sequence first, and where the sequences
 // have equal counts the last tiles of all before the others.
 struct SeqTile {
@@ -173,12 +173,16 @@ __device__ __forceinline__ SeqTile find_tile(const PagedParams& p, int idx, int 
     return SeqTile{b < p.batch ? b : -1, idx - b * each, b * p.per_seq, p.per_seq};
   }
   int base = 0;
-  for (int c = 0; c < p.batch; c += 64) {
-    const int b = min(c + lane, p.batch - 1);
-    const int s0 = clampi(p.starts[b], 0, p.tokens), s1 = clampi(p.starts[b + 1], 0, p.tokens);
-    const int n = c + lane < p.batch ? max(s1 - s0, 0) : 0;
-    const int tiles = (int)(((long long)n * p.group + T - 1) / T);
-    int sum = tiles;
+  for (int c = 0; c < p.batch; c += 256) {
+    int s[5], tiles[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) s[i] = clampi(p.starts[min(c + 4 * lane + i, p.batch)], 0, p.tokens);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      tiles[i] = (int)(((long long)max(s[i + 1] - s[i], 0) * p.group + T - 1) / T);
+      sum += tiles[i];
+    }
+    const int mine = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int below = __shfl_up(sum, o);
@@ -186,10 +190,19 @@ __device__ __forceinline__ SeqTile find_tile(const PagedParams& p, int idx, int 
     }
     const unsigned long long past = __ballot(base + sum > idx);
     if (past) {
-      const int l = __ffsll((long long)past) - 1, count = __builtin_amdgcn_readlane(tiles, l);
-      const int tile = idx - (base + __builtin_amdgcn_readlane(sum, l) - count);
-      return SeqTile{c + l, last_first ? count - 1 - tile : tile, __builtin_amdgcn_readlane(s0, l),
-                     __builtin_amdgcn_readlane(n, l)};
+      const int l = __ffsll((long long)past) - 1;
+      int tile = idx - (base + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
+      int b = c + 4 * l, count = 0, at = 0, n = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        count = __builtin_amdgcn_readlane(tiles[i], l);
+        at = __builtin_amdgcn_readlane(s[i], l);
+        n = __builtin_amdgcn_readlane(s[i + 1], l) - at;
+        if (tile < count) break;
+        tile -= count;
+        ++b;
+      }
+      return SeqTile{b, last_first ? count - 1 - tile : tile, at, n};
     }
     base += __builtin_amdgcn_readlane(sum, 63);
   }

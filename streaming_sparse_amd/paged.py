@@ -218,7 +218,9 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     Arithmetic: scores, maxima, sums and the joins of pieces are float32.  A
     probability meets V in 16 bits: in two parts (hi + lo) where a tile is
     bound by memory, in one where by the matrix pipe (fp16: scaled up by
-    2^7)."""
+    2^7).  Sums reach 2^8 times the values' size times the rows: bf16 values
+    from 2^96 on, and fp16 values within 2^-11 of the type's largest, may come
+    out infinite."""
     device, dtype, dev = q.device, q.dtype, q.get_device()
     code = _TYPES.get(dtype)
     if code is None:

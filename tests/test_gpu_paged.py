@@ -14,6 +14,7 @@ Tolerances, with u = finfo(dtype).eps / 2, half a step of the output type:
 * lse: the scores' error and the sum's, 2^-13 + 2^-12, and a step of its own.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -250,6 +251,74 @@ def test_attention_many_ragged_sequences(device):
     c.check(*c.attend())
 
 
+@pytest.mark.parametrize('count', [255, 257, 700])
+def test_attention_more_sequences_than_a_pass_counts(device, count):
+    """Tiles found among more than 256 sequences, runs of empty ones among them,
+    on either side of a pass's end."""
+    new = [0 if i % 9 < 4 or 250 < i < 256 else 1 + i % 3 for i in range(count)]
+    new[-1] = 2
+    c = Case(device, new, [(13 * i) % 70 for i in range(count)], 2, 1, 33)
+    c.check(*c.attend())
+
+
+def test_attention_in_place_and_two_threads(device):
+    """Output rows over their own query rows, in narrow and wide tiles; two threads
+    that call with different sizes at once, each on a stream of its own."""
+    cs = [Case(device, [1] * 12, [50 * i for i in range(12)], 8, 2, 3000, seed=1),
+          Case(device, [300, 1, 200], [10, 900, 0], 2, 2, 515, seed=2), Case(device, [1], [200], 4, 4, 0, seed=3),
+          Case(device, [700], [30], 8, 1, 0, seed=4)]
+    want = [tuple(x.clone() for x in c.attend()) for c in cs]
+    torch.cuda.synchronize()
+    failed = []
+
+    def calls(order):
+        try:
+            ws, stream = Workspace(), torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for i in order * 5:
+                    out, lse = cs[i].attend(ws=ws)
+                    stream.synchronize()
+                    if not (torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])):
+                        failed.append(i)
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=calls, args=(o,)) for o in ([0, 1, 2, 3], [3, 1, 0, 2])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for c, (out, lse) in zip(cs, want):
+        q = c.q.clone()
+        c.q = q
+        got, got_lse = c.attend(out=q)
+        assert got is q and torch.equal(q, out) and torch.equal(got_lse, lse)
+
+
+def test_attention_graphs_that_share_a_workspace(device):
+    """Two captured calls of different sizes with one workspace, replayed in turn on
+    one stream, between eager calls: each replay equals the eager call."""
+    cs = [Case(device, [1] * 12, [50 * i for i in range(12)], 8, 2, 3000, seed=1),
+          Case(device, [1] * 9, [30 * i for i in range(9)], 8, 2, 4000, seed=2)]
+    ws, graphs, got = Workspace(), [], []
+    want = [tuple(x.clone() for x in c.attend()) for c in cs]
+    for c in cs:
+        c.attend(ws=ws)
+    torch.cuda.synchronize()
+    for c in cs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(c.attend(ws=ws))
+    for _ in range(3):
+        for i in (0, 1, 1, 0):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[i][0], want[i][0]) and torch.equal(got[i][1], want[i][1])
+            cs[i].attend(ws=Workspace())
+            torch.cuda.synchronize()
+
+
 def test_attention_two_streams_at_once(device):
     """Two calls in flight together, each with a workspace of its own."""
     cs = [Case(device, [1] * 12, [50 * i for i in range(12)], 8, 2, 3000, seed=s) for s in (1, 2)]
@@ -328,6 +397,13 @@ def test_append(device, new, before, heads, kv_heads, pairs, interleaved, dtype)
 def test_append_many_tokens(device):
     """Enough tokens for one wave each."""
     c = Case(device, [3000, 1200], [10, 0], 3, 1)
+    append_case(device, c, *kv_parts(c), freqs=freqs(device, 64))
+
+
+def test_append_more_sequences_than_a_wave_counts(device):
+    """Tokens of 300 sequences, empty ones among them."""
+    new = [0 if i % 5 < 2 else 1 + i % 2 for i in range(300)]
+    c = Case(device, new, [(7 * i) % 100 for i in range(300)], 2, 1)
     append_case(device, c, *kv_parts(c), freqs=freqs(device, 64))
 
 
