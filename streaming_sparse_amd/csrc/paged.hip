@@ -654,12 +654,22 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
 // from there the slots at fixed offsets, the raised priority and the loads between
 // the half pages.  The sums as dot products of the rounded pairs, half as many
 // instructions: 2703 us.
-constexpr int kWide = 256, kWideWaves = 8, kSlots = 4;
+constexpr int kWide = 256, kWideWaves = 8;
 constexpr int kTile = 64 * 256;      // a page's K or V rows
 
-// Ring: kSlots pages of K, then of V.
-template <bool F16>
+// Pages of the ring, K of all and then V.  One step, from barrier to barrier, is one
+// page, or with PAIRS two: half as many barriers, from which the waves of a SIMD
+// set out in step (4608 tokens as above 2690 -> 2642 us, 8 x 1536 behind 4608 422 ->
+// 416), but pages come in twos, which a list from memory waits for (16 sequences
+// behind 131001 rows 118 and 123; 20 x 64 tokens, 12 heads, 43 and 47; one of 160, 8
+// heads, behind 30000 42.5 and 44.6; 12 x 200 behind 1500 38.2 and 37.7): so tiles of
+// the prefix by itself, and sequences of up to 192 rows a head, go page by page.
+template <bool PAIRS>
+constexpr int kRing = PAIRS ? 5 : 4;
+
+template <bool F16, bool PAIRS>
 __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
+  constexpr int kSlots = kRing<PAIRS>;
   const int r = lane & 31, hh = lane >> 5;
   int limit;                                  // rows of its sequence that the lane's row sees
   const uint16_t* qp;
@@ -707,7 +717,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     dma_at((const uint8_t*)of_lane(qp, x) + chunk_of(x, lane & 15),
            __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)own_row(4 * jj)));
   }
-  int rows_ahead[kSlots] = {0, 0, 0, 0};    // rows of units i .. i + 3
+  int rows_ahead[5] = {};      // rows of units u .. u + 4
   auto issue = [&](int u) {
     if (u >= end) return 0;
     const Unit x = list.at(p, j, u, lane);
@@ -845,11 +855,15 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   };
 
   if (begin < end) {
+    // The first steps' pages: K and V of one (two), and K of the next; each unit is 2
+    // loads of K, then 2 of V.
+    constexpr int kStep = PAIRS ? 2 : 1, kLater = PAIRS ? 2 : 6;
     if (begin + 3 <= end)
-      loads_left<6>();
+      loads_left<kLater>();
     else
       loads_left<0>();
     clear_rows(begin, rows_ahead[0]);
+    if (PAIRS && begin + 1 < end) clear_rows(begin + 1, rows_ahead[1]);
     meet();
     S = f32x16{};
     if (alive) {
@@ -863,25 +877,38 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     for (int st = 0; st < 4; ++st) ka[st] = kread(0, 1, st);
     int u = begin;
     auto step = [&](auto slot_c) {
+      constexpr std::integral_constant<int, 0> low;
+      constexpr std::integral_constant<int, 1> high;
       f32x16 S1;
-      if (alive) half_step(slot_c, std::integral_constant<int, 0>{}, S, S1, u, rows_ahead[0]);
+      if (alive) half_step(slot_c, low, S, S1, u, rows_ahead[0]);
       rows_ahead[3] = issue(u + 3);
-      if (alive) half_step(slot_c, std::integral_constant<int, 1>{}, S1, S, u + 1, rows_ahead[1]);
-      // next: K of unit u + 2 and V of unit u + 1; each unit is 2 loads of K,
-      // then 2 of V
-      if (u + 3 < end)
-        loads_left<6>();
+      if (alive) half_step(slot_c, high, S1, S, u + 1, rows_ahead[1]);
+      if constexpr (PAIRS) {
+        constexpr std::integral_constant<int, (decltype(slot_c)::value + 1) % kSlots> slot_d;
+        rows_ahead[4] = issue(u + 4);
+        if (alive && u + 1 < end) {
+          half_step(slot_d, low, S, S1, u + 1, rows_ahead[1]);
+          half_step(slot_d, high, S1, S, u + 2, rows_ahead[2]);
+        }
+      }
+      if (u + kStep + 2 < end)
+        loads_left<kLater>();
       else
         loads_left<0>();
-      rows_ahead[0] = rows_ahead[1];
-      rows_ahead[1] = rows_ahead[2];
-      rows_ahead[2] = rows_ahead[3];
-      if (u + 1 < end) clear_rows(u + 1, rows_ahead[0]);
+      u += kStep;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) rows_ahead[i] = rows_ahead[i + kStep];
+      if (u < end) clear_rows(u, rows_ahead[0]);
+      if (PAIRS && u + 1 < end) clear_rows(u + 1, rows_ahead[1]);
       meet();
-      return ++u < end;
+      return u < end;
     };
-    while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{}) &&
-           step(std::integral_constant<int, 2>{}) && step(std::integral_constant<int, 3>{})) {
+    auto slot = [](auto k) { return std::integral_constant<int, decltype(k)::value * kStep % kSlots>{}; };
+    bool more = true;
+    while (more) {
+      more = step(slot(std::integral_constant<int, 0>{})) && step(slot(std::integral_constant<int, 1>{})) &&
+             step(slot(std::integral_constant<int, 2>{})) && step(slot(std::integral_constant<int, 3>{}));
+      if constexpr (PAIRS) more = more && step(slot(std::integral_constant<int, 4>{}));
     }
   }
 
@@ -916,10 +943,10 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
 
 // APART: prefix tiles, then own tiles of 32 rows, eight to a workgroup, a wave
 // each.
-template <bool F16, bool APART>
+template <bool F16, bool APART, bool PAIRS>
 __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p) {
-  __shared__ alignas(16) uint8_t ring[2 * kSlots * kTile];
-  static_assert(sizeof(ring) >= kWideWaves * 2 * kHalf);
+  __shared__ alignas(16) uint8_t ring[2 * kRing<PAIRS> * kTile];
+  static_assert(!APART || sizeof(ring) >= kWideWaves * 2 * kHalf);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int b = blockIdx.x, first = APART ? p.prefix_items : p.own_whole;
   // the longer items first; either kind by itself over the XCDs, but for tiles in
@@ -929,13 +956,13 @@ __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p)
   Job j;
   if constexpr (APART) {
     if (b < first) {
-      if (prefix_job<kWide>(p, item, j)) wide_tile<F16>(p, j, (lds_u8*)ring, lane, wave);
+      if (prefix_job<kWide>(p, item, j)) wide_tile<F16, PAIRS>(p, j, (lds_u8*)ring, lane, wave);
     } else {
       own_items<F16>(p, item, gridDim.x - first, (lds_u8*)ring, lane, wave);
     }
   } else {
     if (own_job<kWide>(p, b < first ? item : first + item, lane, j))
-      wide_tile<F16>(p, j, (lds_u8*)ring, lane, wave);
+      wide_tile<F16, PAIRS>(p, j, (lds_u8*)ring, lane, wave);
   }
 }
 
@@ -1431,8 +1458,12 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
     else
       f16 ? launch(f16_joint, items, 64 * waves) : launch(bf16_joint, items, 64 * waves);
   };
-  if (wide)
-    start(wide_kernel<true, true>, wide_kernel<false, true>, wide_kernel<true, false>, wide_kernel<false, false>);
+  if (wide && (long long)tokens * p.group / batch > 192)
+    start(wide_kernel<true, true, false>, wide_kernel<false, true, false>, wide_kernel<true, false, true>,
+          wide_kernel<false, false, true>);
+  else if (wide)
+    start(wide_kernel<true, true, false>, wide_kernel<false, true, false>, wide_kernel<true, false, false>,
+          wide_kernel<false, false, false>);
   else
     start(narrow_kernel<true, true>, narrow_kernel<false, true>, narrow_kernel<true, false>,
           narrow_kernel<false, false>);
