@@ -647,9 +647,9 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
 // but l ^ 32.  A probability meets V rounded once: the second part would be half
 // as many products again, and the outputs are off by 1.4 times the rounding of
 // probabilities that are normalised first.
-// 4 sequences of 4608 tokens, 12 heads, behind 23040 rows: 2641 us, 1.19 PFLOP/s
-// (an 8192^3 library product 1.40), the matrix pipe busy 62% of the time and the
-// vector pipe 53 at the 1.8 GHz that the chip holds under this load.  Waves of 64
+// 4 sequences of 4608 tokens, 12 heads, behind 23040 rows: 2614 us, 1.20 PFLOP/s
+// (an 8192^3 library product 1.40), the matrix pipe busy 65% of the time and the
+// vector pipe 55 at the 1.65 GHz that the chip holds under this load.  Waves of 64
 // rows, one on a SIMD, read half as much LDS and took 2948 us where these took 2711;
 // from there the slots at fixed offsets, the raised priority and the loads between
 // the half pages.  The sums as dot products of the rounded pairs, half as many
@@ -1286,7 +1286,7 @@ double plan_apart(const Sizes& z, Plan* plan) {
 
 // Every tile over prefix and own pages.  Where their lists are alike and there
 // are more wide tiles than CUs, only those behind the last full round are cut
-// (8 x 1536 tokens, 12 heads, behind 4608: 422 us, 494 uncut); where a causal
+// (8 x 1536 tokens, 12 heads, behind 4608, 422 us and 494 uncut, page by page); where a causal
 // sequence's first tiles have much shorter lists than its last, every list is cut
 // at the same length and the longest come first (2717 tokens, 12 heads: 58 us, 76
 // uncut, 76 in their order; 9 x 2786, 4 heads: 96, 127 in their order).  Sequences

@@ -7,7 +7,7 @@ sequence (a continuation of one history, a candidate of one step) owns pages
 through a row of ``table`` [B, M] int32; a list ``prefix`` of pages lies
 before every sequence.  The new tokens of all sequences are packed, sequence
 b's at rows starts[b] .. starts[b + 1] - 1 of [N, heads, 128] tensors (starts
-None: N / B each).
+[B + 1] int32, from 0 on and not decreasing; None: N / B each).
 
 Every size on the host is a bound only: how many tokens a sequence holds and
 where its rows start are read on the device, so a captured call is replayed
