@@ -54,6 +54,7 @@ struct PagedParams {
   // the longest lists, a causal sequence's last, come first.
   int prefix_items, prefix_tiles, prefix_pieces, prefix_cut, own_tiles, own_whole, own_pieces, own_cut, apart,
       longest_first;
+  int log_rows;       // of an own tile's rows (beside prefix tiles they have 32)
   int row_tiles;      // 32-row tiles of a K/V head's rows, where the prefix is apart
   int own_waves;      // and the waves of a workgroup that take own items then
 };
@@ -154,7 +155,7 @@ struct Job {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
-// Sequence and tile of the idx-th tile of T rows, sequence by sequence (each
+// Sequence and tile of the idx-th tile of T = 2^log_rows rows, sequence by sequence (each
 // sequence's last tile may be short); b = -1 behind the last.  One pass per 256
 // sequences: every lane counts four sequences' tiles, a wave scan sums them.
 // `last_first`: the last tile of each sequence first, and where the sequences
@@ -162,9 +163,10 @@ __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x,
 struct SeqTile {
   int b, tile, start, n;
 };
-__device__ __forceinline__ SeqTile find_tile(const PagedParams& p, int idx, int T, bool last_first, int lane) {
+__device__ __forceinline__ SeqTile find_tile(const PagedParams& p, int idx, int log_rows, bool last_first, int lane) {
+  const int T = 1 << log_rows;
   if (!p.starts) {
-    const int each = (p.per_seq * p.group + T - 1) / T;
+    const int each = (p.per_seq * p.group + T - 1) >> log_rows;
     if (last_first) {
       const int level = idx / p.batch, b = idx - level * p.batch;
       return SeqTile{level < each ? b : -1, each - 1 - level, b * p.per_seq, p.per_seq};
@@ -179,7 +181,7 @@ __device__ __forceinline__ SeqTile find_tile(const PagedParams& p, int idx, int 
     for (int i = 0; i < 5; ++i) s[i] = clampi(p.starts[min(c + 4 * lane + i, p.batch)], 0, p.tokens);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      tiles[i] = (int)(((long long)max(s[i + 1] - s[i], 0) * p.group + T - 1) / T);
+      tiles[i] = (max(s[i + 1] - s[i], 0) * p.group + T - 1) >> log_rows;
       sum += tiles[i];
     }
     const int mine = sum;
@@ -215,8 +217,7 @@ __device__ __forceinline__ int packed_tokens(const PagedParams& p) {
 }
 
 // Prefix item `item` of tiles of T rows; false: no rows.
-template <int T>
-__device__ __forceinline__ bool prefix_job(const PagedParams& p, int item, Job& j) {
+__device__ __forceinline__ bool prefix_job(const PagedParams& p, int item, int T, Job& j) {
   const int tp = item / p.prefix_pieces;
   j.state = item - tp * p.prefix_pieces;
   j.h = tp / p.prefix_tiles;
@@ -231,10 +232,9 @@ __device__ __forceinline__ bool prefix_job(const PagedParams& p, int item, Job& 
   return j.rho0 < j.rho1;
 }
 
-// Own item `item` (behind the prefix items) of tiles of T rows; false: nothing
+// Own item `item` (behind the prefix items) of tiles of 2^log_rows rows; false: nothing
 // to do.
-template <int T>
-__device__ __forceinline__ bool own_job(const PagedParams& p, int item, int lane, Job& j) {
+__device__ __forceinline__ bool own_job(const PagedParams& p, int item, int log_rows, int lane, Job& j) {
   // the tile over all heads, and its piece
   int idx = item, piece = 0, t;
   if (p.longest_first) {
@@ -254,13 +254,13 @@ __device__ __forceinline__ bool own_job(const PagedParams& p, int item, int lane
     j.h = idx / p.own_tiles;
     t = idx - j.h * p.own_tiles;
   }
-  const SeqTile s = find_tile(p, t, T, p.longest_first, lane);
+  const SeqTile s = find_tile(p, t, log_rows, p.longest_first, lane);
   if (s.b < 0 || s.tile < 0) return false;
   j.b = s.b;
   j.n = s.n;
   j.first_token = s.start;
-  j.rho0 = s.start * p.group + s.tile * T;
-  j.rho1 = min(j.rho0 + T, (s.start + s.n) * p.group);
+  j.rho0 = s.start * p.group + (s.tile << log_rows);
+  j.rho1 = min(j.rho0 + (1 << log_rows), (s.start + s.n) * p.group);
   if (j.rho0 >= j.rho1) return false;
   j.length = clampi(p.lengths[j.b], 0, kPage * p.table_pages);
   j.prefix_pages = p.apart ? 0 : (p.prefix_tokens + kPage - 1) / kPage;
@@ -281,16 +281,15 @@ __device__ __forceinline__ bool own_job(const PagedParams& p, int item, int lane
   return piece == 0 || j.begin < units;
 }
 
-// The state that holds row rho (block `blk` of a tile of T rows) of a job, and
-// its place in it.
-template <int T>
+// The state that holds row rho (32-row block `blk` of its tile) of a job, and its
+// place in it.
 __device__ __forceinline__ float* state_of(const PagedParams& p, const Job& j, int rho, int blk, int* col) {
   if (p.apart) {
     *col = rho & 31;
     return p.part + (((long long)j.state * p.kv_heads + j.h) * p.row_tiles + (rho >> 5)) * kState;
   }
   *col = (rho - j.rho0) & 31;
-  return p.part + ((long long)j.state * (T / 32) + blk) * kState;
+  return p.part + ((long long)j.state * (1 << (p.log_rows - 5)) + blk) * kState;
 }
 
 // The pages of a job's list, walked upwards: lane l holds page base + l of the
@@ -340,7 +339,7 @@ struct PageList {
 // probabilities meet V in two parts (hi + lo), so that no rounding of theirs
 // shows in the output.  One token of 32 heads on 8 K/V heads behind 60000 rows:
 // 52.8 us, 4.7 TB/s (a large copy 5.1).
-constexpr int kNarrow = 32, kNarrowWaves = 4;
+constexpr int kNarrow = 32, kLogNarrow = 5, kNarrowWaves = 4;
 constexpr int kHalf = 32 * 256;      // 32 rows of K or V
 
 template <int N>
@@ -372,13 +371,12 @@ __device__ __forceinline__ void meet() {
 
 // Writes what a lane holds of a row to the row's state: 16 groups of 4 dims (8 c +
 // 4 hh of row rho = j.rho0 + 32 blk + lane % 32), the maximum M and the sum l.
-template <int T>
 __device__ __forceinline__ void write_state(const PagedParams& p, const Job& j, const f32x16 (&O)[4], float M, float l,
                                             int blk, int lane) {
   const int rho = j.rho0 + 32 * blk + (lane & 31), hh = lane >> 5;
   if (rho >= j.rho1) return;
   int col;
-  float* st = state_of<T>(p, j, rho, blk, &col);
+  float* st = state_of(p, j, rho, blk, &col);
   // the sums of an empty state are not read
 #pragma unroll
   for (int c = 0; c < 16 && j.begin < j.end; ++c) {
@@ -530,7 +528,7 @@ __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, 
   const float l = half_sum(ls);
   const float mine = m == -INFINITY ? m : m - kLift<F16>;
   if constexpr (NW == 1) {
-    write_state<kNarrow>(p, j, O, mine, l, 0, e);      // beside prefix tiles, so never the last word
+    write_state(p, j, O, mine, l, 0, e);      // beside prefix tiles, so never the last word
   } else {
     // the waves' states into one: every wave hands over m, l and its 32 x 128
     // sums, [dim tile][j][lane] of 4 floats, two dim tiles at a time (8 KB a wave;
@@ -579,7 +577,7 @@ __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, 
     if (rho >= j.rho1) return;
     if (j.state >= 0) {
       int col;
-      float* st = state_of<kNarrow>(p, j, rho, 0, &col);
+      float* st = state_of(p, j, rho, 0, &col);
 #pragma unroll
       for (int i = 0; i < kItems; ++i)
         *reinterpret_cast<f32x4*>(st + ((2 * (wave * kItems + i) + he) * 32 + col) * 4) = R[i];
@@ -614,7 +612,7 @@ __device__ __forceinline__ void own_items(const PagedParams& p, int group, int g
   const int all = p.kv_heads * p.own_tiles * p.own_pieces;
   Job j;
   for (long long own = group * p.own_waves + wave; own < all; own += (long long)groups * p.own_waves) {
-    if (own_job<kNarrow>(p, (int)own, lane, j)) narrow_tile<F16, 1>(p, j, ring, lane, wave);
+    if (own_job(p, (int)own, kLogNarrow, lane, j)) narrow_tile<F16, 1>(p, j, ring, lane, wave);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // its rows are read before the next ones come
   }
 }
@@ -629,17 +627,17 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
   Job j;
   if constexpr (APART) {
     if (b < first) {
-      if (prefix_job<kNarrow>(p, item, j)) narrow_tile<F16, kNarrowWaves>(p, j, (lds_u8*)ring, lane, wave);
+      if (prefix_job(p, item, kNarrow, j)) narrow_tile<F16, kNarrowWaves>(p, j, (lds_u8*)ring, lane, wave);
     } else {
       own_items<F16>(p, item, gridDim.x - first, (lds_u8*)ring, lane, wave);
     }
   } else {
-    if (own_job<kNarrow>(p, item, lane, j)) narrow_tile<F16, kNarrowWaves>(p, j, (lds_u8*)ring, lane, wave);
+    if (own_job(p, item, kLogNarrow, lane, j)) narrow_tile<F16, kNarrowWaves>(p, j, (lds_u8*)ring, lane, wave);
   }
 }
 
 // ---------------------------------------------------------------------------
-// Wide tiles: 256 rows.  Bound by the matrix pipe and the vector work of the
+// Wide tiles: 256 rows, or 128.  Bound by the matrix pipe and the vector work of the
 // softmax together: eight waves, two on a SIMD, so that one's products run under
 // the other's exponentials; each holds 32 rows with their sums in registers and
 // walks every key, and all share the pages.  S^T = K Q^T and O^T += V^T P^T on
@@ -654,7 +652,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
 // from there the slots at fixed offsets, the raised priority and the loads between
 // the half pages.  The sums as dot products of the rounded pairs, half as many
 // instructions: 2703 us.
-constexpr int kWide = 256, kWideWaves = 8;
+constexpr int kWide = 256, kHalfWide = 128, kWideWaves = 8;
 constexpr int kTile = 64 * 256;      // a page's K or V rows
 
 // Pages of the ring, K of all and then V.  One step, from barrier to barrier, is one
@@ -917,7 +915,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   asm volatile("" : "+v"(e));
   const float M = m == -INFINITY ? m : m - kLift<F16>, l = half_sum(ls);
   if (j.state >= 0) {
-    write_state<kWide>(p, j, O, M, l, wave, e);
+    write_state(p, j, O, M, l, wave, e);
     return;
   }
   const int x = e & 31, he = e >> 5, rho = j.rho0 + 32 * wave + x;
@@ -956,12 +954,12 @@ __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p)
   Job j;
   if constexpr (APART) {
     if (b < first) {
-      if (prefix_job<kWide>(p, item, j)) wide_tile<F16, PAIRS>(p, j, (lds_u8*)ring, lane, wave);
+      if (prefix_job(p, item, kWide, j)) wide_tile<F16, PAIRS>(p, j, (lds_u8*)ring, lane, wave);
     } else {
       own_items<F16>(p, item, gridDim.x - first, (lds_u8*)ring, lane, wave);
     }
   } else {
-    if (own_job<kWide>(p, b < first ? item : first + item, lane, j))
+    if (own_job(p, b < first ? item : first + item, p.log_rows, lane, j))
       wide_tile<F16, PAIRS>(p, j, (lds_u8*)ring, lane, wave);
   }
 }
@@ -1022,13 +1020,13 @@ __device__ __forceinline__ Gathered<N> gather(const float* st, long long step, i
   return got;
 }
 
-// Joins the pieces' states of 32 rows of a K/V head, 528 bytes a row and piece: block (h, rows 32 T .., group)
-// where the prefix is apart (T_ROWS 0), else (split tile of T_ROWS rows, block of
-// 32, group).  Bound by the latency of its loads.  Few pieces: a group is 32 dims, a
-// wave gathers 8 of them over all pieces.  MANY: a group is 16 dims, which the
-// four waves gather over a quarter of the pieces each; their sums meet in LDS (32
-// pieces, 8 rows: 3.7 us).
-template <bool F16, int T_ROWS, bool MANY>
+// Joins the pieces' states of 32 rows of a K/V head, 528 bytes a row and piece:
+// block (h, rows 32 T .., group) where the prefix is apart, else (split tile,
+// block of 32, group).  Bound by the latency of its loads.  Few pieces: a group is
+// 32 dims, a wave gathers 8 of them over all pieces.  MANY: a group is 16 dims,
+// which the four waves gather over a quarter of the pieces each; their sums meet
+// in LDS (32 pieces, 8 rows: 3.7 us).
+template <bool F16, bool APART, bool MANY>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedParams p) {
   constexpr int kGroups = MANY ? 8 : 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -1036,7 +1034,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedParams p) {
   int h, rho, end, pieces;
   long long step;                 // floats from a piece to the next
   const float* st;
-  if constexpr (T_ROWS == 0) {
+  if constexpr (APART) {
     h = block / p.row_tiles;
     rho = 32 * (block - h * p.row_tiles) + r;
     end = packed_tokens(p) * p.group;
@@ -1044,17 +1042,16 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedParams p) {
     step = (long long)p.kv_heads * p.row_tiles * kState;
     st = p.part + (long long)block * kState;
   } else {
-    constexpr int kBlocks = T_ROWS / 32;
-    const int t = block / kBlocks, blk = block - t * kBlocks;
+    const int log_blocks = p.log_rows - 5, t = block >> log_blocks, blk = block - (t << log_blocks);
     Job j;
     // the tile's first piece
-    if (!own_job<T_ROWS>(p, p.longest_first ? t : p.own_whole + t * p.own_pieces, lane, j) || j.state < 0) return;
+    if (!own_job(p, p.longest_first ? t : p.own_whole + t * p.own_pieces, p.log_rows, lane, j) || j.state < 0) return;
     h = j.h;
     rho = j.rho0 + 32 * blk + r;
     end = j.rho1;
     pieces = (j.prefix_pages + j.own_pages + p.own_cut - 1) / p.own_cut;
-    step = (long long)kBlocks * kState;
-    st = p.part + ((long long)t * p.own_pieces * kBlocks + blk) * kState;
+    step = (long long)kState << log_blocks;
+    st = p.part + (((long long)t * p.own_pieces << log_blocks) + blk) * kState;
   }
   const bool live = rho < end;
   float M, L;
@@ -1116,7 +1113,8 @@ struct Plan {
   }
   long long bytes(int kv_heads) const { return 4ll * kState * states(kv_heads); }
   // workgroups of the launches, and whether a grid holds them (2^32 threads)
-  int waves() const { return rows == kWide ? kWideWaves : kNarrowWaves; }
+  bool wide() const { return rows > kNarrow; }
+  int waves() const { return wide() ? kWideWaves : kNarrowWaves; }
   long long prefix_items(int kv_heads) const { return 1ll * kv_heads * prefix_tiles * prefix_pieces; }
   long long own_items(int kv_heads) const { return own_whole + split_tiles(kv_heads) * own_pieces; }
   long long items(int kv_heads) const {
@@ -1134,26 +1132,30 @@ struct Plan {
   }
 };
 
-// Estimates, in us, that the pieces are chosen by, from captured calls (224, 96 and
-// 32 workgroups, 17 and 65 pages each): a workgroup's start and end and a page of its
-// tile, a state written and read again, pages from memory.  A wide tile's page
-// takes 0.93 to 0.98 us with up to 128 rows (a wave on each SIMD), 1.35 with 192,
-// with 256 1.62 where all CUs work and 1.32 where few do (the clock falls under the
-// matrix pipe's load); a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A
-// page that no other tile reads takes 1.1 and 1.2 at least, which is what one
-// workgroup draws from memory.  Waves by themselves: a CU draws a page in 0.85 us (8
-// of them one each in 6.8), a wave one in 3.5, and an item begins and ends in 5.
-// Tables are taken to be 0.6 to 0.7 full, which only shifts the choice.
+// Estimates, in us, that the pieces are chosen by, from captured calls (224, 96
+// and 32 workgroups, 17 and 65 pages each): a workgroup's start and end and a page
+// of its tile, a state written and read again, pages from memory.  A wide tile's
+// page takes 0.93 to 0.98 us with up to 128 rows (a wave on each SIMD), 1.35 with
+// 192, with 256 1.62 where all CUs work and 1.32 where few do (the clock falls
+// under the matrix pipe's load), 7% less with two pages between barriers; a narrow
+// tile's 0.47, 0.72 with two workgroups on a CU.  A page that no other tile reads
+// takes 1.1 and 1.2 at least, which is what one workgroup draws from memory.
+// Waves by themselves: a CU draws a page in 0.85 us (8 of them one each in 6.8), a
+// wave one in 3.5, and an item begins and ends in 5. Tables are taken to be 0.6 to
+// 0.7 full, which only shifts the choice.
 constexpr double kJoinStart = 3.0, kSoloPage = 0.85, kSoloLatency = 3.5, kSoloStart = 3.0, kSoloItem = 5.0;
-double start_time(int T, double rows) { return T == kWide ? 6.0 + 5.0 * rows / kWide : 7.0; }
-double tile_page(int T, double rows, double active, double cus, double unshared) {
+double start_time(int T, double rows, bool singly) {
+  return T == kNarrow ? 7.0 : singly ? 6.0 + 5.0 * rows / kWide : 5.0 + 3.0 * rows / kWide;
+}
+double tile_page(int T, double rows, double active, double cus, double unshared, bool singly) {
   const double busy = active / cus;
   double page;
   if (T == kNarrow) {
     page = 0.47 + 0.25 * std::min(1.0, std::max(0.0, busy - 1.0));
   } else {
     const double second = std::max(0.0, std::ceil(rows / 32) - 4) / 4;     // SIMDs with two waves
-    page = second > 0 ? 1.3 + 0.3 * std::min(1.0, busy) * second * second : 0.95;
+    const double few = singly ? 1.3 : 1.2, more = singly ? 0.3 : 0.25;
+    page = second > 0 ? few + more * std::min(1.0, busy) * second * second : 0.95;
   }
   return page + unshared * std::max(0.0, (T == kNarrow ? 1.2 : 1.1) - page);
 }
@@ -1245,9 +1247,9 @@ double plan_apart(const Sizes& z, Plan* plan) {
     if (c > 1 && 2 * c > prefix_pages) break;
     int cut;
     const int pieces = cut_in(prefix_pages, c, &cut);
-    const double t = start_time(T, live) + cut * tile_page(T, std::min<double>(rows, T),
+    const double t = start_time(T, live, true) + cut * tile_page(T, std::min<double>(rows, T),
                                                            std::min(tiles * pieces, (double)slots), z.cus,
-                                                           plan->prefix_tiles == 1 ? 1.0 : 0.0);
+                                                           plan->prefix_tiles == 1 ? 1.0 : 0.0, true);
     const double rounds = std::ceil(tiles * pieces / slots), left = rounds * slots - tiles * pieces;
     for (int d : kCuts) {
       if (d > 16 || (d > 1 && 2 * d > z.table_pages)) break;
@@ -1291,11 +1293,13 @@ double plan_apart(const Sizes& z, Plan* plan) {
 // at the same length and the longest come first (2717 tokens, 12 heads: 58 us, 76
 // uncut, 76 in their order; 9 x 2786, 4 heads: 96, 127 in their order).  Sequences
 // of up to 32 rows a K/V head take narrow tiles (40 x 3 tokens: 16.3 us, 22.7 with
-// wide ones).
-double plan_joint(const Sizes& z, Plan* plan) {
+// wide ones); others tiles of 256 rows or, where those leave CUs idle, of 128, whose
+// waves have a SIMD each (12 x 200 tokens, 8 heads, behind 1500: 33.6 us, 38.4 with
+// 256; 3 x 601 behind 126: 18.4 and 23.0; 5 x 531 behind 4389 86.4 and 82.7).
+double plan_joint(const Sizes& z, int T, Plan* plan) {
   const double per_seq = (double)z.rows() / z.batch;
-  const int T = per_seq <= kNarrow ? kNarrow : kWide, units = z.table_pages + z.prefix_pages();
-  const bool wide = T == kWide;
+  const int units = z.table_pages + z.prefix_pages();
+  const bool wide = T > kNarrow, singly = per_seq <= 192;       // pages one by one
   const int slots = wide ? z.cus : 2 * z.cus;
   plan->rows = T;
   plan->row_tiles = plan->prefix_tiles = plan->prefix_pieces = plan->prefix_cut = 0;
@@ -1309,7 +1313,7 @@ double plan_joint(const Sizes& z, Plan* plan) {
   const double tiles = (double)(own_tiles - whole);
   const double full = std::min<double>(per_seq, T);         // rows of the fullest tile
   const double live = per_seq / std::ceil(per_seq / T);     // and of the mean one
-  const double start = start_time(T, live);
+  const double start = start_time(T, live, singly);
   // the part of all lists' pages that come from memory, and of a list that no other
   // tile reads
   const double read = std::min(1.0, z.kv_heads * (z.prefix_pages() + (double)z.batch * z.table_pages) /
@@ -1325,7 +1329,7 @@ double plan_joint(const Sizes& z, Plan* plan) {
     double time, states = 0.0;
     if (plan->longest_first) {
       const double mean = units - 0.5 * spread, each = std::max(1.0, mean / cut + (c > 1 ? 0.5 : 0.0));
-      const double page = tile_page(T, full, std::min(tiles * each, (double)slots), z.cus, unshared);
+      const double page = tile_page(T, full, std::min(tiles * each, (double)slots), z.cus, unshared, singly);
       const double longest = start + cut * page;
       time = tiles * each <= slots ? longest
                                    : std::max(longest, tiles * (each * start + mean * page) / slots + 0.5 * longest);
@@ -1333,7 +1337,7 @@ double plan_joint(const Sizes& z, Plan* plan) {
     } else {
       const double active = std::min(tiles * pieces, (double)slots);
       time = std::ceil(tiles * pieces / slots) *
-             (start + std::max(cut * tile_page(T, full, active, z.cus, unshared),
+             (start + std::max(cut * tile_page(T, full, active, z.cus, unshared, singly),
                                page_time(read * active * cut, active / z.cus)));
       states = pieces > 1 ? tiles * pieces : 0.0;
     }
@@ -1345,7 +1349,7 @@ double plan_joint(const Sizes& z, Plan* plan) {
     }
   }
   plan->own_whole = (int)(plan->own_pieces == 1 ? own_tiles : whole);
-  return least + (double)(whole / z.cus) * (start + units * tile_page(T, full, slots, z.cus, unshared));
+  return least + (double)(whole / z.cus) * (start + units * tile_page(T, full, slots, z.cus, unshared, singly));
 }
 
 // The plan of a call's sizes (z.cus is filled in).  A thread keeps its last one:
@@ -1356,9 +1360,18 @@ int make_plan(Sizes z, Plan* plan) {
   static thread_local Sizes last_sizes{};
   static thread_local Plan last_plan;
   if (!(z == last_sizes)) {
-    Plan joint, apart;
-    const double t = plan_joint(z, &joint);
-    last_plan = z.batch > 1 && z.prefix_tokens > 0 && plan_apart(z, &apart) < t ? apart : joint;
+    Plan joint, other;
+    const bool narrow = z.rows() <= (long long)kNarrow * z.batch;
+    double t = plan_joint(z, narrow ? kNarrow : kWide, &joint);
+    auto consider = [&](double time) {
+      if (time < t) {
+        joint = other;
+        t = time;
+      }
+    };
+    if (!narrow) consider(plan_joint(z, kHalfWide, &other));
+    if (z.batch > 1 && z.prefix_tokens > 0) consider(plan_apart(z, &other));
+    last_plan = joint;
     last_sizes = z;
   }
   *plan = last_plan;
@@ -1433,6 +1446,7 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   p.table_pages = table_pages;
   p.causal = (flags & 2) != 0;
   p.scale_log2 = scale * kLog2e;
+  p.log_rows = plan.rows == kNarrow ? 5 : plan.rows == kHalfWide ? 7 : 8;
   p.row_tiles = plan.row_tiles;
   p.own_waves = plan.own_waves;
   p.prefix_tiles = plan.prefix_tiles;
@@ -1447,7 +1461,7 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   p.prefix_items = (int)plan.prefix_items(kv_heads);
   const long long items = plan.items(kv_heads), joins = plan.joins(kv_heads);
   const int waves = plan.waves();
-  const bool wide = plan.rows == kWide, many = plan.many();
+  const bool wide = plan.wide(), many = plan.many();
   const bool f16 = flags & 1;
   auto launch = [&](auto kernel, long long blocks, int threads) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, p);
@@ -1475,14 +1489,11 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   };
   if (joins > 0) {
     if (plan.apart())
-      join(join_kernel<true, 0, false>, join_kernel<false, 0, false>, join_kernel<true, 0, true>,
-           join_kernel<false, 0, true>);
-    else if (!wide)
-      join(join_kernel<true, kNarrow, false>, join_kernel<false, kNarrow, false>, join_kernel<true, kNarrow, true>,
-           join_kernel<false, kNarrow, true>);
+      join(join_kernel<true, true, false>, join_kernel<false, true, false>, join_kernel<true, true, true>,
+           join_kernel<false, true, true>);
     else
-      join(join_kernel<true, kWide, false>, join_kernel<false, kWide, false>, join_kernel<true, kWide, true>,
-           join_kernel<false, kWide, true>);
+      join(join_kernel<true, false, false>, join_kernel<false, false, false>, join_kernel<true, false, true>,
+           join_kernel<false, false, true>);
   }
   return (int)hipGetLastError();
 }

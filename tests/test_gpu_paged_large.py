@@ -34,6 +34,9 @@ CASES = [
     pytest.param(1, 200, True, 50, 8, 2, 30000, True, BF16, id='joint_wide_many_pieces'),
     pytest.param(20, 64, True, 900, 12, 12, 0, True, FP16, id='joint_wide_few_rows'),
     pytest.param(3, 150, False, 700, 2, 1, 5, False, BF16, id='joint_wide_one_or_two_tiles'),
+    pytest.param(3, 601, True, 7, 8, 8, 126, True, FP16, id='half_wide_whole'),
+    pytest.param(1, 1265, True, 134, 12, 4, 248, True, BF16, id='half_wide_causal_cut'),
+    pytest.param(2, 185, False, 725, 12, 3, 15, False, BF16, id='half_wide_pieces'),
     pytest.param(2, 700, True, 0, 48, 48, 1000, False, BF16, id='joint_wide_rounds'),
     pytest.param(1, 2000, True, 100, 12, 12, 10, True, BF16, id='causal_cut'),
     pytest.param(3, 1500, False, 10, 24, 24, 3, True, FP16, id='causal_whole'),
