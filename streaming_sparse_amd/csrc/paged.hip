@@ -939,8 +939,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   if (p.lse && he == 0 && rho < j.rho1) p.lse[(long long)token * p.heads + hq] = lse_of(M, l);
 }
 
-// APART: prefix tiles, then own tiles of 32 rows, eight to a workgroup, a wave
-// each.
+// APART: prefix tiles, then own tiles of 32 rows, a wave each.
 template <bool F16, bool APART, bool PAIRS>
 __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p) {
   __shared__ alignas(16) uint8_t ring[2 * kRing<PAIRS> * kTile];
