@@ -60,7 +60,9 @@ int ssa_paged_append(const void* q, long long q_token_stride, long long q_head_s
  *   out = softmax(scale q . k) v,  lse [tokens, heads] fp32 (or NULL) = ln sum
  * exp(scale q . k).  A query that sees no row has out 0 and lse -infinity.
  * Rows of out and lse from starts[batch] on are left as they were.  Pages
- * outside [0, pages) count as absent: none of their rows is seen.  Values in
+ * outside [0, pages), and those behind the table's end where a length passes
+ * it, count as absent: none of their rows is seen, nor does any other row's
+ * place change.  Values in
  * rows of a page that no query sees (behind a sequence's or the prefix's end)
  * may be anything, NaN included; one that some query of the call sees must be
  * finite for the others to come out finite.  out may be q itself.

@@ -69,7 +69,8 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, starts
     shared = [] if prefix is None else prefix.tolist()
 
     def rows(pages, count):
-        got = []
+        # cache rows, -1 where a page is absent; none of those behind the list
+        got, count = [], min(count, PAGE * len(pages))
         for i in range(-(-count // PAGE)):
             if 0 <= pages[i] < P:
                 got += [PAGE * pages[i] + r for r in range(min(PAGE, count - PAGE * i))]

@@ -148,7 +148,7 @@ struct Job {
   int h;              // K/V head
   int rho0, rho1;     // rows
   int state;          // where its states go, -1: it writes out
-  int b, n, length, first_token;   // the rows' sequence: new tokens, rows in the cache, first packed token
+  int b, n, length, first_token;   // the rows' sequence: new tokens, rows with them, first packed token
   int prefix_pages, own_pages;     // pages of the list
   int begin, end;                  // this piece of it
 };
@@ -262,11 +262,16 @@ __device__ __forceinline__ bool own_job(const PagedParams& p, int item, int log_
   j.rho0 = s.start * p.group + (s.tile << log_rows);
   j.rho1 = min(j.rho0 + (1 << log_rows), (s.start + s.n) * p.group);
   if (j.rho0 >= j.rho1) return false;
-  j.length = clampi(p.lengths[j.b], 0, kPage * p.table_pages);
+  // A length may pass the table (tokens whose rows it does not hold): the causal
+  // limit goes by the length, which beyond `held + n` changes nothing more, the pages
+  // by the rows that the table holds.
+  const int held = kPage * p.table_pages;
+  j.length = clampi(p.lengths[j.b], 0, held + j.n);
   j.prefix_pages = p.apart ? 0 : (p.prefix_tokens + kPage - 1) / kPage;
   // rows the tile's last query sees
   int seen = j.length;
-  if (p.causal) seen = clampi(j.length - j.n + (j.rho1 - 1) / p.group - j.first_token + 1, 0, j.length);
+  if (p.causal) seen = j.length - j.n + (j.rho1 - 1) / p.group - j.first_token + 1;
+  seen = clampi(seen, 0, min(j.length, held));
   j.own_pages = (seen + kPage - 1) / kPage;
   const int units = j.prefix_pages + j.own_pages;
   const int cut = item < p.own_whole || p.own_pieces == 1 ? max(units, 1) : p.own_cut;

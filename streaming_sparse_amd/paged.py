@@ -206,8 +206,8 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     among them.  Query i of n attends the prefix and its sequence's rows j <
     lengths[b], with `causal` only j <= lengths[b] - n + i.  A query that
     sees nothing gets zeros (and lse -inf).  Rows from starts[B] on are left
-    as they were.  Pages outside the cache (-1) count as absent; rows that no
-    query sees may hold anything, while a value row that some query of the
+    as they were.  Pages outside the cache (-1) and, where a length passes it,
+    behind the table's end count as absent; rows that no query sees may hold anything, while a value row that some query of the
     call sees must be finite for the others to come out finite.
 
     scale defaults to 128 ** -0.5.  Returns out [N, H, 128], or (out, lse)

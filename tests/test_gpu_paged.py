@@ -164,6 +164,27 @@ def test_attention_absent_pages(device):
     c.check(*c.attend())
 
 
+@pytest.mark.parametrize('causal', [True, False], ids=['causal', 'full'])
+@pytest.mark.parametrize('new,before,heads,kv_heads,prefix,drop', [
+    pytest.param([4], [126], 2, 2, 0, 1, id='narrow'),
+    pytest.param([1, 5, 2], [70, 190, 3], 4, 2, 130, 2, id='narrow_shared'),
+    pytest.param([1] * 40, [64 + 7 * i for i in range(40)], 2, 1, 300, 3, id='wide_shared'),
+    pytest.param([300, 40], [10, 250], 2, 2, 70, 2, id='wide'),
+    pytest.param([257], [3], 1, 1, 0, 4, id='wide_few_rows_left'),
+])
+def test_attention_lengths_past_the_table(device, new, before, heads, kv_heads, prefix, drop, causal):
+    """Tokens that were not written, their rows outside the table: the others keep
+    the rows that they see, whatever the length is."""
+    c = Case(device, new, before, heads, kv_heads, prefix)
+    c.table = c.table[:, :max(1, c.table.shape[1] - drop)].contiguous()
+    assert int(c.lengths.max()) > 64 * c.table.shape[1]
+    c.check(*c.attend(causal), causal)
+    # no query misses a row that it should see, up to the largest length there is
+    # (the longest sequence's, whose rows fill the table)
+    c.lengths[c.lengths.argmax()] = 2 ** 31 - 1
+    c.check(*c.attend(causal), causal)
+
+
 def test_attention_wide_table_and_repeated_pages(device):
     """A table wider than any sequence, and sequences that share own pages."""
     c = Case(device, [1, 1, 1], [100, 140, 20], 4, 4, 64, width=40)
