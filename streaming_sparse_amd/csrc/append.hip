@@ -201,7 +201,10 @@ extern "C" int ssa_paged_append(const void* q, long long q_token_stride, long lo
       pages <= 0 || table_pages <= 0 || (!starts && tokens % batch) || (flags & ~3))
     return (int)hipErrorInvalidValue;
   if (pairs < 0 || pairs > kHeadDim / 2 || (!interleaved && pairs % 8) || (pairs > 0 && !freqs) || axes < 1 ||
-      axes > 3 || axis0 < 0 || axis1 < 0 || axis0 + axis1 > pairs || (axes > 1 && !positions && pairs > 0))
+      axes > 3 || axis0 < 0 || axis1 < 0 || axis0 > pairs - axis1 || (axes > 1 && !positions && pairs > 0))
+    return (int)hipErrorInvalidValue;
+  // pairs behind the counts turn on the next axis, which positions must hold
+  if (positions && pairs > 0 && ((axes == 1 && axis0 != pairs) || (axes == 2 && axis0 + axis1 != pairs)))
     return (int)hipErrorInvalidValue;
   if (!k || !v || !cache_k || !cache_v || !table || !held || (heads > 0 && (!q || !q_out)))
     return (int)hipErrorInvalidValue;

@@ -143,6 +143,18 @@ def test_append_abi_rejects():
         assert append_call(**{'tokens': 2, **change}) == INVALID, change
 
 
+@built
+def test_append_abi_rejects_pairs_beyond_the_axes():
+    """Positions hold `axes` numbers a token: no pair may turn on one behind them,
+    which for the last token would lie outside the tensor."""
+    for change in (dict(axis0=63), dict(axis0=0), dict(axis0=32, axis1=32), dict(axis0=40, axis1=20),
+                   dict(axes=2, axis0=32, axis1=31), dict(axes=2, axis0=0, axis1=0), dict(axes=2, axis0=63)):
+        assert append_call(**{'tokens': 2, 'positions': 4096, **change}) == INVALID, change
+    for change in (dict(), dict(axes=2, axis0=32, axis1=32), dict(axes=2, axis0=64), dict(axes=3, axis0=22, axis1=21),
+                   dict(axes=3, axis0=0)):
+        assert append_call(**{'positions': 4096, **change}) == 0, change
+
+
 def attention_call(**change):
     a = dict(q=4096, q_tok=512, q_head=128, ck=4096, cv=4096, kv_tok=256, kv_head=128, prefix=4096, prefix_tokens=100,
              table=4096, lengths=4096, starts=None, out=4096, o_tok=512, o_head=128, lse=None, tokens=2, batch=2,
