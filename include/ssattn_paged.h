@@ -38,10 +38,12 @@ extern "C" {
  * positions[t, axis] (int32 [tokens, axes], axes 1..3, wanted for axes > 1):
  * the first axis0 pairs turn on axis 0, the next axis1 on axis 1, the others on
  * axis 2; with positions the counts must reach the last of fewer axes: axis0 =
- * pairs for one, axis0 + axis1 = pairs for two.  Angles are formed in float64; each result is rounded once.
+ * pairs for one, axis0 + axis1 = pairs for two.  Angles are formed in float64;
+ * each result is rounded once.
  *
  * q [tokens, heads, 128] goes to q_out (which may be q itself); heads = 0: no
- * queries.  k and v must not overlap the cache rows written.  tokens < 2^26. */
+ * queries.  k and v must not overlap the cache rows written.  tokens is at most
+ * 2^26 - 4. */
 int ssa_paged_append(const void* q, long long q_token_stride, long long q_head_stride, void* q_out,
                      long long out_token_stride, long long out_head_stride, const void* k, long long k_token_stride,
                      long long k_head_stride, const void* v, long long v_token_stride, long long v_head_stride,

@@ -196,9 +196,10 @@ extern "C" int ssa_paged_append(const void* q, long long q_token_stride, long lo
                                 int pages, int table_pages, int pairs, int axis0, int axis1, int axes, int flags,
                                 hipStream_t stream) {
   const bool interleaved = flags & 2;
-  // a grid holds less than 2^32 threads, 2^26 tokens
-  if (tokens < 0 || tokens >= 1 << 26 || batch <= 0 || heads < 0 || kv_heads <= 0 || heads + 2ll * kv_heads > 65536 ||
-      pages <= 0 || table_pages <= 0 || (!starts && tokens % batch) || (flags & ~3))
+  // a grid holds less than 2^32 threads
+  constexpr int kMostTokens = kWaves * (int)(((1ll << 32) - 1) / (64 * kWaves));
+  if (tokens < 0 || tokens > kMostTokens || batch <= 0 || heads < 0 || kv_heads <= 0 ||
+      heads + 2ll * kv_heads > 65536 || pages <= 0 || table_pages <= 0 || (!starts && tokens % batch) || (flags & ~3))
     return (int)hipErrorInvalidValue;
   if (pairs < 0 || pairs > kHeadDim / 2 || (!interleaved && pairs % 8) || (pairs > 0 && !freqs) || axes < 1 ||
       axes > 3 || axis0 < 0 || axis1 < 0 || axis0 > pairs - axis1 || (axes > 1 && !positions && pairs > 0))

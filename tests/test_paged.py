@@ -155,6 +155,13 @@ def test_append_abi_rejects_pairs_beyond_the_axes():
         assert append_call(**{'positions': 4096, **change}) == 0, change
 
 
+@built
+@pytest.mark.parametrize('tokens', [(1 << 26) - 3, (1 << 26) - 2, (1 << 26) - 1])
+def test_append_abi_rejects_tokens_that_no_grid_holds(tokens):
+    """2^24 workgroups of 256 threads are 2^32 threads."""
+    assert append_call(tokens=tokens, batch=1) == INVALID
+
+
 def attention_call(**change):
     a = dict(q=4096, q_tok=512, q_head=128, ck=4096, cv=4096, kv_tok=256, kv_head=128, prefix=4096, prefix_tokens=100,
              table=4096, lengths=4096, starts=None, out=4096, o_tok=512, o_head=128, lse=None, tokens=2, batch=2,
