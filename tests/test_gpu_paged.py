@@ -233,6 +233,44 @@ def test_attention_masked_nan_key(device):
         assert torch.equal(got[:c.N - 2], want[:c.N - 2]) and torch.isnan(got[c.N - 2:]).all()
 
 
+@pytest.mark.parametrize('new,before,heads,kv_heads,prefix', [
+    pytest.param([1], [3], 2, 2, 1300, id='narrow_pieces'),
+    pytest.param([1, 1, 2], [70, 0, 100], 4, 4, 700, id='narrow_shared'),
+    pytest.param([1] * 40, [64 + 7 * i for i in range(40)], 4, 1, 1300, id='wide_shared'),
+    pytest.param([150, 40], [10, 250], 2, 1, 700, id='wide'),
+    pytest.param([40], [1500], 2, 1, 0, id='wide_pieces'),
+])
+def test_attention_nan_and_infinite_scores(device, new, before, heads, kv_heads, prefix):
+    """A key that makes a score NaN or +infinity makes NaN of every row that sees it;
+    one that makes all of a row's scores but one -infinity leaves that row its
+    one value; both in any piece of the list, in the middle of a tile."""
+    c = Case(device, new, before, heads, kv_heads, prefix)
+    c.q[:] = c.q.abs() + 0.5
+    b, n = len(new) - 1, new[-1]
+    at = before[-1] // 2
+    row = 64 * int(c.table[b, at // 64]) + at % 64
+    keep = c.k[0, row].clone()
+    clean = tuple(x.clone() for x in c.attend())
+    for value in (math.nan, math.inf):
+        c.k[0, row, :, 7] = value
+        out, lse = c.attend()
+        assert torch.isnan(out[c.N - n:]).all()
+        assert torch.equal(out[:c.N - n], clean[0][:c.N - n]) and torch.equal(lse[:c.N - n], clean[1][:c.N - n])
+        c.k[0, row] = keep
+    # every key that the last sequence sees but one at -infinity
+    held = before[-1] + n
+    rows = [64 * int(p) + r for i, p in enumerate(c.prefix.tolist()) for r in range(min(64, prefix - 64 * i))] + \
+        [64 * int(c.table[b, i // 64]) + i % 64 for i in range(held)]
+    c.k[0, rows, :, 7] = -math.inf
+    c.k[0, row] = keep
+    out, lse = c.attend()
+    z = (c.q[c.N - n:].double().reshape(n, kv_heads, -1, 128) * c.k[0, row].double()[None, :, None]).sum(-1) * 128 ** -0.5
+    want = c.v[0, row].double()[None, :, None].expand(n, kv_heads, heads // kv_heads, 128).reshape(n, heads, 128)
+    u = torch.finfo(c.dtype).eps / 2
+    assert ((out[c.N - n:].double() - want).abs() <= (2 * u + 2.0 ** -12) * want.abs()).all()
+    assert ((lse[c.N - n:].double() - z.reshape(n, heads)).abs() <= 2.0 ** -13 + 2.0 ** -20).all()
+
+
 def test_attention_layouts(device):
     """K and V side by side in one cache, head-major and broadcast queries, out in
     place of q, a table whose entries behind the sequence are garbage."""

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import paged as oracle
-from streaming_sparse_amd import _lib, paged
+from streaming_sparse_amd import _lib, build, paged
 from streaming_sparse_amd.attention import Workspace
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -101,6 +101,15 @@ def test_no_tokens_is_no_call():
     assert paged.append(a['k'], a['v'], a['ck'], a['cv'], a['table'], a['held'], q=a['q']).shape == (0, 4, 128)
     out, lse = paged.attention(a['q'], a['ck'], a['cv'], None, 0, a['table'], a['held'], Workspace(), want_lse=True)
     assert out.shape == (0, 4, 128) and lse.shape == (0, 4)
+
+
+def test_paged_sources_keep_nan_semantics():
+    """Rows that no query sees may hold NaN, and a NaN that is seen reaches the
+    output: neither source may be compiled as if there were none."""
+    for source in ("paged.hip", "append.hip"):
+        flags = build.FLAGS + build.EXTRA.get(source, [])
+        assert source in build.SOURCES
+        assert not {"-fno-honor-nans", "-ffinite-math-only", "-ffast-math", "-Ofast"} & set(flags), source
 
 
 built = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libssattn.so not built")
