@@ -94,3 +94,31 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, starts
                 out[t, h] = p @ vv if len(at) else 0.0
                 spread[t, h] = p @ vv.abs() if len(at) else 0.0
     return out, lse, spread
+
+
+
+def error_limit(want, p2, p2v2, dtype, parts):
+    """What the root of the summed squared errors of outputs `want` [..., 128] may
+    be, given sum p^2 [...] and sum p^2 v^2 [..., 128] over their normalised
+    probabilities, each of which meets V in `parts` 16-bit parts.
+
+    * A result rounded once is off by an error uniform within half a step: mean
+      square step^2 / 12, the sum's standard deviation sqrt(4 / 5) of the root of
+      the squared means' sum.  Six of those are allowed, here and below.
+    * One part: a probability is off by at most eps / 2 of itself, mean square
+      below eps^2 / 12, one error for all 128 dims: their quadratic form over a row
+      has the mean eps^2 / 12 sum p^2 v^2 and a variance of at most twice its square
+      times 1 / 128 + sum p^2.
+    * The rest, as a part of each probability and of the output: scores' 128
+      float32 roundings of sums below 16 (root mean square 2^-18), exponents
+      and exponentials (2^-20), a second part's rounding (below 2^-16 in bf16, 2^-22
+      in fp16), sums of up to 2^15 terms (2^-17): 2^-15.
+    Errors of different origin add up as their roots at most."""
+    info = torch.finfo(dtype)
+    step = torch.exp2(torch.floor(torch.log2(want.abs().clamp_min(info.smallest_normal)))) * info.eps
+    e = step * step / 12
+    limit = (e.sum() + 6 * (0.8 * (e * e).sum()).sqrt()).sqrt()
+    if parts == 1:
+        e = p2v2.sum(-1) * info.eps ** 2 / 12
+        limit = limit + (e.sum() + 6 * (2 * (e * e * (1 / 128 + p2)).sum()).sqrt()).sqrt()
+    return limit + 2.0 ** -15 * (p2v2.sum() + (want * want).sum()).sqrt()

@@ -647,9 +647,17 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
 // the other's exponentials; each holds 32 rows with their sums in registers and
 // walks every key, and all share the pages.  S^T = K Q^T and O^T += V^T P^T on
 // 32 x 32 x 16 products: a lane holds one query, its softmax needs no other lane
-// but l ^ 32.  A probability meets V rounded once: the second part would be half
-// as many products again, and the outputs are off by 1.4 times the rounding of
-// probabilities that are normalised first.
+// but l ^ 32.
+// A probability meets V in one 16-bit part or in two (TWO).  One: it is rounded,
+// and the outputs' error is 1.4 times that of their own rounding (of bf16 outputs
+// 0.00235 relative, with two parts 0.00166; fp16 0.000286 and 0.000207).  The second
+// part is half as many products again: 4 x 4608 tokens behind 23040 rows 2686 and
+// 3722 us, 8 x 1536 behind 4608 422 and 573, six prompts of up to 901 behind 8192
+// 464 and 635.  So it is the caller's to ask for where a sequence fills tiles by
+// itself.  Tiles of a prefix apart hold the steps of many sequences, each of which
+// alone would take a narrow tile: they take two parts unless asked otherwise, so
+// that a step's precision does not change with the batch (64 x 1 behind 16384 48.3
+// and 51.4 us, 16 x 1 behind 131001 118.9 and 123.6, 24 x 5 behind 5003 27.9 and 32.1).
 // 4 sequences of 4608 tokens, 12 heads, behind 23040 rows: 2614 us, 1.20 PFLOP/s
 // (an 8192^3 library product 1.40), the matrix pipe busy 65% of the time and the
 // vector pipe 55 at the 1.65 GHz that the chip holds under this load.  Waves of 64
@@ -670,7 +678,7 @@ constexpr int kTile = 64 * 256;      // a page's K or V rows
 template <bool PAIRS>
 constexpr int kRing = PAIRS ? 5 : 4;
 
-template <bool F16, bool PAIRS>
+template <bool F16, bool PAIRS, bool TWO>
 __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
   constexpr int kSlots = kRing<PAIRS>;
   const int r = lane & 31, hh = lane >> 5;
@@ -813,7 +821,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     constexpr int slot = decltype(slot_c)::value, half = decltype(half_c)::value;
     constexpr int nslot = (slot + half) % kSlots, nhalf = half ^ 1;            // the next half page
     constexpr int aslot = (slot + 1) % kSlots, ahalf = half;                   // and the one after
-    u32x4 va[2][4], pb[2];
+    u32x4 va[2][4], pb[2], pl[2];       // pl: the second parts
     float P[16];
     auto vread = [&](int ks, int dt) {
       const lds_u8* a = vat[dt] + slot * kTile + half * (kTile / 2) + 4096 * ks;
@@ -822,7 +830,14 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     auto expo = [&](int i) {
       P[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(Sc[i], p.scale_log2, nb));
       ls += P[i];
-      if (i & 1) pb[i >> 3][(i & 7) >> 1] = pack2<F16>(P[i - 1], P[i]);
+      if (!(i & 1)) return;
+      if constexpr (TWO) {
+        const u32x2 x = split2<F16>(P[i - 1], P[i]);
+        pb[i >> 3][(i & 7) >> 1] = x[0];
+        pl[i >> 3][(i & 7) >> 1] = x[1];
+      } else {
+        pb[i >> 3][(i & 7) >> 1] = pack2<F16>(P[i - 1], P[i]);
+      }
     };
     Sn = f32x16{};
     __builtin_amdgcn_s_setprio(1);
@@ -839,6 +854,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
       O[dt] = mma<F16>(va[0][dt], pb[0], O[dt]);
+      if constexpr (TWO) O[dt] = mma<F16>(va[0][dt], pl[0], O[dt]);
       va[1][dt] = vread(1, dt);
       expo(8 + 2 * dt);
       expo(9 + 2 * dt);
@@ -847,6 +863,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
       O[dt] = mma<F16>(va[1][dt], pb[1], O[dt]);
+      if constexpr (TWO) O[dt] = mma<F16>(va[1][dt], pl[1], O[dt]);
       ka[dt] = kread(aslot, ahalf, dt);
     }
     mx = half_max(lane_max(Sn));
@@ -944,8 +961,9 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   if (p.lse && he == 0 && rho < j.rho1) p.lse[(long long)token * p.heads + hq] = lse_of(M, l);
 }
 
-// APART: prefix tiles, then own tiles of 32 rows, a wave each.
-template <bool F16, bool APART, bool PAIRS>
+// APART: prefix tiles, then own tiles of 32 rows, a wave each.  TWO: a probability
+// meets V in two parts.
+template <bool F16, bool APART, bool PAIRS, bool TWO>
 __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p) {
   __shared__ alignas(16) uint8_t ring[2 * kRing<PAIRS> * kTile];
   static_assert(!APART || sizeof(ring) >= kWideWaves * 2 * kHalf);
@@ -958,13 +976,13 @@ __global__ __launch_bounds__(64 * kWideWaves, 1) void wide_kernel(PagedParams p)
   Job j;
   if constexpr (APART) {
     if (b < first) {
-      if (prefix_job(p, item, kWide, j)) wide_tile<F16, PAIRS>(p, j, (lds_u8*)ring, lane, wave);
+      if (prefix_job(p, item, kWide, j)) wide_tile<F16, PAIRS, TWO>(p, j, (lds_u8*)ring, lane, wave);
     } else {
       own_items<F16>(p, item, gridDim.x - first, (lds_u8*)ring, lane, wave);
     }
   } else {
     if (own_job(p, b < first ? item : first + item, p.log_rows, lane, j))
-      wide_tile<F16, PAIRS>(p, j, (lds_u8*)ring, lane, wave);
+      wide_tile<F16, PAIRS, TWO>(p, j, (lds_u8*)ring, lane, wave);
   }
 }
 
@@ -1141,8 +1159,9 @@ struct Plan {
 // of its tile, a state written and read again, pages from memory.  A wide tile's
 // page takes 0.93 to 0.98 us with up to 128 rows (a wave on each SIMD), 1.35 with
 // 192, with 256 1.62 where all CUs work and 1.32 where few do (the clock falls
-// under the matrix pipe's load), 7% less with two pages between barriers; a narrow
-// tile's 0.47, 0.72 with two workgroups on a CU.  A page that no other tile reads
+// under the matrix pipe's load), 7% less with two pages between barriers; in two
+// parts (a prefix apart) 1.15 to 2.0 (64 x 1 token behind 16384 cut by the figures of
+// one part 55.9 us, by these 51.4; 128 x 1 behind 4096 69.3 and 58.4); a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A page that no other tile reads
 // takes 1.1 and 1.2 at least, which is what one workgroup draws from memory.
 // Waves by themselves: a CU draws a page in 0.85 us (8 of them one each in 6.8), a
 // wave one in 3.5, and an item begins and ends in 5. Tables are taken to be 0.6 to
@@ -1151,15 +1170,15 @@ constexpr double kJoinStart = 3.0, kSoloPage = 0.85, kSoloLatency = 3.5, kSoloSt
 double start_time(int T, double rows, bool singly) {
   return T == kNarrow ? 7.0 : singly ? 6.0 + 5.0 * rows / kWide : 5.0 + 3.0 * rows / kWide;
 }
-double tile_page(int T, double rows, double active, double cus, double unshared, bool singly) {
+double tile_page(int T, double rows, double active, double cus, double unshared, bool singly, bool two) {
   const double busy = active / cus;
   double page;
   if (T == kNarrow) {
     page = 0.47 + 0.25 * std::min(1.0, std::max(0.0, busy - 1.0));
   } else {
     const double second = std::max(0.0, std::ceil(rows / 32) - 4) / 4;     // SIMDs with two waves
-    const double few = singly ? 1.3 : 1.2, more = singly ? 0.3 : 0.25;
-    page = second > 0 ? few + more * std::min(1.0, busy) * second * second : 0.95;
+    const double few = two ? 1.7 : singly ? 1.3 : 1.2, more = singly ? 0.3 : 0.25;
+    page = second > 0 ? few + more * std::min(1.0, busy) * second * second : two ? 1.15 : 0.95;
   }
   return page + unshared * std::max(0.0, (T == kNarrow ? 1.2 : 1.1) - page);
 }
@@ -1253,7 +1272,7 @@ double plan_apart(const Sizes& z, Plan* plan) {
     const int pieces = cut_in(prefix_pages, c, &cut);
     const double t = start_time(T, live, true) + cut * tile_page(T, std::min<double>(rows, T),
                                                            std::min(tiles * pieces, (double)slots), z.cus,
-                                                           plan->prefix_tiles == 1 ? 1.0 : 0.0, true);
+                                                           plan->prefix_tiles == 1 ? 1.0 : 0.0, true, true);
     const double rounds = std::ceil(tiles * pieces / slots), left = rounds * slots - tiles * pieces;
     for (int d : kCuts) {
       if (d > 16 || (d > 1 && 2 * d > z.table_pages)) break;
@@ -1333,7 +1352,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
     double time, states = 0.0;
     if (plan->longest_first) {
       const double mean = units - 0.5 * spread, each = std::max(1.0, mean / cut + (c > 1 ? 0.5 : 0.0));
-      const double page = tile_page(T, full, std::min(tiles * each, (double)slots), z.cus, unshared, singly);
+      const double page = tile_page(T, full, std::min(tiles * each, (double)slots), z.cus, unshared, singly, false);
       const double longest = start + cut * page;
       time = tiles * each <= slots ? longest
                                    : std::max(longest, tiles * (each * start + mean * page) / slots + 0.5 * longest);
@@ -1341,7 +1360,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
     } else {
       const double active = std::min(tiles * pieces, (double)slots);
       time = std::ceil(tiles * pieces / slots) *
-             (start + std::max(cut * tile_page(T, full, active, z.cus, unshared, singly),
+             (start + std::max(cut * tile_page(T, full, active, z.cus, unshared, singly, false),
                                page_time(read * active * cut, active / z.cus)));
       states = pieces > 1 ? tiles * pieces : 0.0;
     }
@@ -1353,7 +1372,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
     }
   }
   plan->own_whole = (int)(plan->own_pieces == 1 ? own_tiles : whole);
-  return least + (double)(whole / z.cus) * (start + units * tile_page(T, full, slots, z.cus, unshared, singly));
+  return least + (double)(whole / z.cus) * (start + units * tile_page(T, full, slots, z.cus, unshared, singly, false));
 }
 
 // The plan of a call's sizes (z.cus is filled in).  A thread keeps its last one:
@@ -1404,7 +1423,7 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
                         float* lse, int tokens, int batch, int heads, int kv_heads, int pages, int table_pages,
                         float scale, int flags, void* workspace, long long workspace_bytes, hipStream_t stream) {
   if (!sizes_fit(tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr) || pages <= 0 ||
-      (flags & ~3) || !(scale > 0.0f && scale < INFINITY))
+      (flags & ~(3 | 3 << 3)) || flags >> 3 == 3 || !(scale > 0.0f && scale < INFINITY))
     return (int)hipErrorInvalidValue;
   if (!q || !cache_k || !cache_v || !table || !lengths || !out || (prefix_tokens > 0 && !prefix))
     return (int)hipErrorInvalidValue;
@@ -1467,24 +1486,29 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   const int waves = plan.waves();
   const bool wide = plan.wide(), many = plan.many();
   const bool f16 = flags & 1;
+  // parts of a probability in wide tiles: as asked, else two with the prefix apart
+  const int parts = flags >> 3;
+  const bool two = parts ? parts == 2 : plan.apart();
   auto launch = [&](auto kernel, long long blocks, int threads) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, p);
   };
-  auto start = [&](auto f16_apart, auto bf16_apart, auto f16_joint, auto bf16_joint) {
-    if (plan.apart())
-      f16 ? launch(f16_apart, items, 64 * waves) : launch(bf16_apart, items, 64 * waves);
-    else
-      f16 ? launch(f16_joint, items, 64 * waves) : launch(bf16_joint, items, 64 * waves);
+  auto start = [&](auto f16_kernel, auto bf16_kernel) {
+    f16 ? launch(f16_kernel, items, 64 * waves) : launch(bf16_kernel, items, 64 * waves);
   };
-  if (wide && (long long)tokens * p.group / batch > 192)
-    start(wide_kernel<true, true, false>, wide_kernel<false, true, false>, wide_kernel<true, false, true>,
-          wide_kernel<false, false, true>);
-  else if (wide)
-    start(wide_kernel<true, true, false>, wide_kernel<false, true, false>, wide_kernel<true, false, false>,
-          wide_kernel<false, false, false>);
+  const bool pairs = !plan.apart() && (long long)tokens * p.group / batch > 192;
+  if (!wide && plan.apart())
+    start(narrow_kernel<true, true>, narrow_kernel<false, true>);
+  else if (!wide)
+    start(narrow_kernel<true, false>, narrow_kernel<false, false>);
+  else if (plan.apart())
+    two ? start(wide_kernel<true, true, false, true>, wide_kernel<false, true, false, true>)
+        : start(wide_kernel<true, true, false, false>, wide_kernel<false, true, false, false>);
+  else if (pairs)
+    two ? start(wide_kernel<true, false, true, true>, wide_kernel<false, false, true, true>)
+        : start(wide_kernel<true, false, true, false>, wide_kernel<false, false, true, false>);
   else
-    start(narrow_kernel<true, true>, narrow_kernel<false, true>, narrow_kernel<true, false>,
-          narrow_kernel<false, false>);
+    two ? start(wide_kernel<true, false, false, true>, wide_kernel<false, false, false, true>)
+        : start(wide_kernel<true, false, false, false>, wide_kernel<false, false, false, false>);
   auto join = [&](auto f16_few, auto bf16_few, auto f16_many, auto bf16_many) {
     if (many)
       f16 ? launch(f16_many, joins, 64 * kJoinWaves) : launch(bf16_many, joins, 64 * kJoinWaves);

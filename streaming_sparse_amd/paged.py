@@ -25,6 +25,7 @@ from .legacy_components import HEAD_DIM
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _INT, _F64 = torch.int32, torch.float64
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_PARTS = {None: 0, True: 1 << 3, False: 2 << 3}        # single_av as the call's flags
 
 
 # The checks below stand in the path of a call of a few microseconds, so each
@@ -194,7 +195,7 @@ _BYTES = {}
 
 
 def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, workspace, *, starts=None, causal=True,
-              scale=None, want_lse=False, out=None):
+              scale=None, want_lse=False, out=None, single_av=None):
     """Attention of every sequence's new queries over the shared prefix and the
     sequence's own rows; the prefix is read for all sequences together.
 
@@ -207,8 +208,9 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     lengths[b], with `causal` only j <= lengths[b] - n + i.  A query that
     sees nothing gets zeros (and lse -inf).  Rows from starts[B] on are left
     as they were.  Pages outside the cache (-1) and, where a length passes it,
-    behind the table's end count as absent; rows that no query sees may hold anything, while a value row that some query of the
-    call sees must be finite for the others to come out finite.
+    behind the table's end count as absent; rows that no query sees may hold
+    anything, while a value row that some query of the call sees must be
+    finite for the others to come out finite.
 
     scale defaults to 128 ** -0.5.  Returns out [N, H, 128], or (out, lse)
     with want_lse, lse [N, H] float32 the log of the sum of exponentials:
@@ -216,11 +218,15 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     given (q itself is allowed; otherwise it must not overlap what is read).
 
     Arithmetic: scores, maxima, sums and the joins of pieces are float32.  A
-    probability meets V in 16 bits: in two parts (hi + lo) where a tile is
-    bound by memory, in one where by the matrix pipe (fp16: scaled up by
-    2^7).  Sums reach 2^8 times the values' size times the rows: bf16 values
-    from 2^96 on, and fp16 values within 2^-11 of the type's largest, may come
-    out infinite."""
+    probability meets V in 16 bits (fp16: scaled up by 2^7): in two parts (hi
+    + lo), which leave the output its own rounding, or in one, with which its
+    error is 1.4 times as large.  ``single_av=False``: two parts throughout;
+    the default None: two, but one where the sequences bring more than 32 rows
+    a K/V head (their mean) and walk the prefix in tiles of their own, which
+    the matrix pipe bounds (two parts take 1.4 times as long there);
+    ``single_av=True``: one in all tiles of more than 32 rows.  Sums reach 2^8 times the values' size times the rows: bf16
+    values from 2^96 on, and fp16 values within 2^-11 of the type's largest,
+    may come out infinite."""
     device, dtype, dev = q.device, q.dtype, q.get_device()
     code = _TYPES.get(dtype)
     if code is None:
@@ -238,6 +244,9 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
         prefix_ptr = _ints(prefix, "prefix", prefix.shape, dev)
     elif prefix_tokens < 0:
         raise ValueError("prefix_tokens must not be negative")
+    parts = _PARTS.get(single_av)
+    if parts is None:
+        raise ValueError("single_av must be None, True or False")
     if scale is None:
         scale = _SCALE
     elif not 0.0 < scale < math.inf:
@@ -259,7 +268,7 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
         _launch("ssa_paged_attention", device, dev, q_ptr, q_tok, q_head, cache_k.data_ptr(), cache_v.data_ptr(),
                 kv_tok, kv_head, prefix_ptr, prefix_tokens, table_ptr, len_ptr, starts_ptr, out_ptr, o_tok, o_head,
                 None if lse is None else lse.data_ptr(), n, batch, h, g, rows >> 6, width, scale,
-                code | 2 if causal else code, part, need)
+                (code | 2 if causal else code) | parts, part, need)
     return (out, lse) if want_lse else out
 
 

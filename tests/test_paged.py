@@ -218,3 +218,57 @@ def test_oracle_rotation_is_complex_multiplication():
     halves = torch.cat([x[..., 0::2], x[..., 1::2]], -1)
     want = torch.cat([w[..., 0::2], w[..., 1::2]], -1)
     assert torch.allclose(oracle.rotate(halves, pos, f, (64,), False), want, atol=1e-12)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=['bf16', 'fp16'])
+@pytest.mark.parametrize('keys', [300, 2000, 30250])
+def test_error_limit_tells_wrong_outputs(keys, dtype):
+    """The limit holds for outputs rounded once, with probabilities in two parts or
+    one, and is passed by far by mistakes planted in the float64 form: a page
+    of V left out, two half pages exchanged, and, against the limit of two
+    parts over a few thousand outputs, probabilities in one part."""
+    g = torch.Generator().manual_seed(keys)
+    rows = 16
+    q, k, v = (torch.randn(n, 128, generator=g).to(dtype).double() for n in (rows, keys, keys))
+    p = (q @ k.t() * 128 ** -0.5).softmax(-1)
+    want, p2, p2v2 = p @ v, (p * p).sum(-1), (p * p) @ (v * v)
+
+    # as a tile forms them: beside the row's largest, in fp16 2^7 times as large
+    unit = p.amax(-1, keepdim=True) / (128 if dtype is torch.float16 else 1)
+
+    def part(x):
+        return (x / unit).to(dtype).double() * unit
+
+    def size(out, rows=slice(None)):
+        return (out.to(dtype).double() - want)[rows].norm()
+
+    def limit(parts, r=slice(None)):
+        return oracle.error_limit(want[r], p2[r], p2v2[r], dtype, parts)
+
+    hi = part(p)
+    both = hi + part(p - hi)
+    assert size(both @ v) <= limit(2) and size(hi @ v) <= limit(1)
+    assert size(hi @ v) > limit(2)
+    for r in range(rows):
+        assert size(both @ v, [r]) <= limit(2, [r]) and size(hi @ v, [r]) <= limit(1, [r])
+    at = keys // 128 * 64
+    lost, moved = v.clone(), v.clone()
+    lost[at:at + 64] = 0
+    moved[at:at + 32], moved[at + 32:at + 64] = v[at + 32:at + 64], v[at:at + 32]
+    for bad in (lost, moved):
+        for r in range(rows):
+            assert size(p @ bad, [r]) > 3 * limit(1, [r])
+
+
+def test_attention_rejects_what_is_no_precision():
+    a = args()
+    for value in ('two', 2, 0.5):
+        with pytest.raises(ValueError):
+            paged.attention(a['q'], a['ck'], a['cv'], a['prefix'], 100, a['table'], a['held'], Workspace(),
+                            single_av=value)
+
+
+@built
+def test_attention_abi_rejects_unknown_flags():
+    for flags in (3 << 3, 1 << 5, 4 | 1 << 3, -1):
+        assert attention_call(flags=flags) == INVALID, flags
