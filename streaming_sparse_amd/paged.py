@@ -80,6 +80,11 @@ def _written(x, name, dtype, dev):
     return got
 
 
+def _in_place(ptr, tok, head, n, h, start):
+    """Whether n x h rows at `ptr` are those of a contiguous tensor at `start`."""
+    return ptr == start and (n < 2 or tok == h * HEAD_DIM) and (h < 2 or head == HEAD_DIM)
+
+
 def _ints(x, name, shape, dev):
     if x.dtype is not _INT or x.shape != shape or not x.is_contiguous() or x.get_device() != dev:
         raise ValueError(f"{name} must be a contiguous int32 {list(shape)} tensor on the rows' device")
@@ -134,7 +139,8 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
 
     q_out: where the rotated queries go (q itself is allowed; otherwise it must
     not overlap what is read); else a buffer owned by `workspace` that the next
-    call overwrites, or, without one, a new tensor."""
+    call, of whatever size, overwrites (so q may be the last call's result as
+    it stands, but no other part of that buffer), or, without one, a new tensor."""
     device, dtype, dev = k.device, k.dtype, k.get_device()
     code = _TYPES.get(dtype)
     if code is None:
@@ -172,9 +178,15 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
         if nq != n or h == 0:
             raise ValueError("q must be [N, H, 128]")
         if q_out is None:
-            q_out = torch.empty((n, h, HEAD_DIM), dtype=dtype, device=device) if workspace is None else \
-                workspace.tensor('paged_q', (n, h, HEAD_DIM), device, dtype)
-            o_tok, o_head, out_ptr = h * HEAD_DIM, HEAD_DIM, q_out.data_ptr()
+            o_tok, o_head = h * HEAD_DIM, HEAD_DIM
+            if workspace is None:
+                q_out = torch.empty((n, h, HEAD_DIM), dtype=dtype, device=device)
+                out_ptr = q_out.data_ptr()
+            else:
+                q_out, out_ptr, end = workspace.rows('paged_q', (n, h, HEAD_DIM), device, dtype)
+                if out_ptr <= k_ptr < end or out_ptr <= v_ptr < end or \
+                        out_ptr <= q_ptr < end and not _in_place(q_ptr, q_tok, q_head, n, h, out_ptr):
+                    raise ValueError("q, k or v lies in the workspace's buffer for the rotated queries: give q_out")
         else:
             no, ho, o_tok, o_head, out_ptr = _written(q_out, "q_out", dtype, dev)
             if no != n or ho != h:
@@ -214,8 +226,9 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
 
     scale defaults to 128 ** -0.5.  Returns out [N, H, 128], or (out, lse)
     with want_lse, lse [N, H] float32 the log of the sum of exponentials:
-    buffers owned by `workspace` and overwritten by the next call, or `out` as
-    given (q itself is allowed; otherwise it must not overlap what is read).
+    buffers owned by `workspace` and overwritten by the next call, of whatever
+    size, or `out` as given (q itself is allowed; otherwise it must not overlap
+    what is read).
 
     Arithmetic: scores, maxima, sums and the joins of pieces are float32.  A
     probability meets V in 16 bits (fp16: scaled up by 2^7): in two parts (hi
@@ -252,13 +265,17 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     elif not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive")
     if out is None:
-        out = workspace.tensor('paged_out', (n, h, HEAD_DIM), device, dtype)
-        o_tok, o_head, out_ptr = h * HEAD_DIM, HEAD_DIM, out.data_ptr()
+        out, out_ptr, end = workspace.rows('paged_out', (n, h, HEAD_DIM), device, dtype)
+        o_tok, o_head = h * HEAD_DIM, HEAD_DIM
+        if out_ptr <= q_ptr < end and not _in_place(q_ptr, q_tok, q_head, n, h, out_ptr):
+            raise ValueError("q lies in the workspace's buffer for the output: give out")
     else:
         no, ho, o_tok, o_head, out_ptr = _written(out, "out", dtype, dev)
         if no != n or ho != h:
             raise ValueError("out must have q's shape")
-    lse = workspace.tensor('paged_lse', (n, h), device, torch.float32) if want_lse else None
+    lse = lse_ptr = None
+    if want_lse:
+        lse, lse_ptr, _ = workspace.rows('paged_lse', (n, h), device, torch.float32)
     if n:
         key = (n, batch, h, g, prefix_tokens, width, starts is None, causal, dev)
         need = _BYTES.get(key)
@@ -267,7 +284,7 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
         part = workspace.tensor('paged_part', (need,), device, torch.uint8).data_ptr() if need else None
         _launch("ssa_paged_attention", device, dev, q_ptr, q_tok, q_head, cache_k.data_ptr(), cache_v.data_ptr(),
                 kv_tok, kv_head, prefix_ptr, prefix_tokens, table_ptr, len_ptr, starts_ptr, out_ptr, o_tok, o_head,
-                None if lse is None else lse.data_ptr(), n, batch, h, g, rows >> 6, width, scale,
+                lse_ptr, n, batch, h, g, rows >> 6, width, scale,
                 (code | 2 if causal else code) | parts, part, need)
     return (out, lse) if want_lse else out
 

@@ -404,6 +404,28 @@ def test_attention_workspace_of_many_sizes(device):
     assert sizes and len(sizes) <= 8 and all(x & (x - 1) == 0 for x in sizes)
 
 
+def test_results_of_many_sizes_in_one_workspace(device):
+    """Steps whose token count changes from call to call, their results in one
+    workspace's shared buffers, the rotated queries passed on from there; a
+    result turned again in place."""
+    ws, f = Workspace(), freqs(device, 64)
+    for n in (5, 8, 3, 9, 16, 1, 7):
+        c = Case(device, [2] * n, [40] * n, 4, 2, 600)
+        k, v = kv_parts(c)
+        q = paged.append(k, v, c.k, c.v, c.table, c.held, q=c.q, freqs=f, workspace=ws)
+        want = paged.append(k, v, c.k, c.v, c.table, c.held, q=c.q, freqs=f)
+        assert torch.equal(q, want)
+        c.q = q
+        out, lse = c.attend(ws=ws)
+        c.q = want
+        c.check(out, lse)
+        again = paged.append(k, v, c.k, c.v, c.table, c.held, q=q, freqs=f, workspace=ws)
+        assert again.data_ptr() == q.data_ptr()
+        assert torch.equal(again, paged.append(k, v, c.k, c.v, c.table, c.held, q=want, freqs=f))
+    counts = [sum(key[0] == name for key in ws.entries) for name in ('paged_q', 'paged_out', 'paged_lse')]
+    assert counts == [4, 4, 4]              # of 2, 8, 16 and 32 rows
+
+
 def test_attention_sizes_that_no_grid_holds(device):
     """2^25 tiles of 256 threads are refused before anything is launched."""
     size = _lib.lib().ssa_paged_attention_workspace_bytes

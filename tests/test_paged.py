@@ -112,6 +112,59 @@ def test_paged_sources_keep_nan_semantics():
         assert not {"-fno-honor-nans", "-ffinite-math-only", "-ffast-math", "-Ofast"} & set(flags), source
 
 
+@pytest.fixture
+def no_launch(monkeypatch):
+    """Calls without their launch: what the Python side alone does."""
+    launched = []
+    monkeypatch.setattr(paged, '_launch', lambda name, device, dev, *given: launched.append((name, given)))
+    monkeypatch.setattr(paged, '_workspace_bytes', lambda key, device: 0)
+    monkeypatch.setattr(paged, '_BYTES', {})
+    return launched
+
+
+def test_calls_of_many_sizes_share_a_few_buffers(no_launch):
+    """A workspace that sees every token count up to 600 keeps one buffer per power
+    of two for queries, outputs and lse, less than four times the largest together."""
+    a, ws = args(B=1, n=600, pages=20), Workspace()
+    for n in (*range(1, 601), 37, 600, 1):
+        q, k, v = a['q'][:n], a['k'][:n], a['v'][:n]
+        turned = paged.append(k, v, a['ck'], a['cv'], a['table'], a['held'], q=q, workspace=ws)
+        out, lse = paged.attention(turned, a['ck'], a['cv'], None, 0, a['table'], a['held'], ws, want_lse=True)
+        assert turned.shape == out.shape == q.shape and lse.shape == q.shape[:2]
+        assert turned.is_contiguous() and out.is_contiguous() and lse.is_contiguous()
+        assert turned.data_ptr() != out.data_ptr()
+    assert len(no_launch) == 2 * 603 and len(ws.entries) == 3 * 11
+    assert ws.bytes() < 4 * 600 * 4 * (2 * 256 + 4)
+
+
+def test_rows_in_the_buffer_that_is_written(no_launch):
+    """A result that lies in the workspace may come back as it stands, whatever the
+    next call's size; other parts of its buffer are refused."""
+    a, ws = args(B=1, n=12, H=2, pages=20), Workspace()
+    turn = lambda q, k, v: paged.append(k, v, a['ck'], a['cv'], a['table'], a['held'], q=q, workspace=ws)
+    see = lambda q: paged.attention(q, a['ck'], a['cv'], None, 0, a['table'], a['held'], ws)
+    q = turn(a['q'], a['k'], a['v'])
+    assert turn(q, a['k'], a['v']).data_ptr() == q.data_ptr()
+    assert turn(q[:9], a['k'][:9], a['v'][:9]).data_ptr() == q.data_ptr()
+    for bad in (q[1:10], q.as_strided((9, 2, 128), (128, 128, 1)), q[:9, 1:].expand(9, 2, 128)):
+        with pytest.raises(ValueError):
+            turn(bad, a['k'][:9], a['v'][:9])
+    for part in (q[:9], q[3:12]):
+        with pytest.raises(ValueError):
+            turn(a['q'][:9], part, a['v'][:9])
+        with pytest.raises(ValueError):
+            turn(a['q'][:9], a['k'][:9], part)
+    out = see(q)
+    assert see(out).data_ptr() == see(out[:9]).data_ptr() == out.data_ptr()
+    for bad in (out[1:10], out.as_strided((9, 2, 128), (128, 128, 1)), out[:9, 1:].expand(9, 2, 128)):
+        with pytest.raises(ValueError):
+            see(bad)
+    one = args(B=1, n=1, H=1, G=1, pages=2)
+    q = paged.append(one['k'], one['v'], one['ck'], one['cv'], one['table'], one['held'], q=one['q'], workspace=ws)
+    with pytest.raises(ValueError):
+        paged.append(q, one['v'], one['ck'], one['cv'], one['table'], one['held'], q=one['q'], workspace=ws)
+
+
 built = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libssattn.so not built")
 
 
