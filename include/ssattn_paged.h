@@ -34,9 +34,9 @@ extern "C" {
  *
  * The pairs j < pairs (at most 64) of query and key rows turn by position *
  * freqs[j] (float64, radians): elements (2j, 2j + 1) with flags bit 1, else (j,
- * j + pairs), pairs then a multiple of 8.  The position is first + at, or
- * positions[t, axis] (int32 [tokens, axes], axes 1..3, wanted for axes > 1):
- * the first axis0 pairs turn on axis 0, the next axis1 on axis 1, the others on
+ * j + pairs), pairs then a multiple of 8.  The position is first + at (first
+ * within 2^53), or positions[t, axis] (int32 [tokens, axes], axes 1..3, wanted
+ * for axes > 1): the first axis0 pairs turn on axis 0, the next axis1 on axis 1, the others on
  * axis 2; with positions the counts must reach the last of fewer axes: axis0 =
  * pairs for one, axis0 + axis1 = pairs for two.  Angles are formed in float64;
  * each result is rounded once.

@@ -6,9 +6,10 @@
 //   y1 = x1 cos - x2 sin,  y2 = x1 sin + x2 cos
 // over the elements (2j, 2j + 1) (interleaved) or (j, j + pairs) (halves);
 // the other elements are copied bit for bit.  The angle is formed in turns in
-// float64 and reduced to half a turn there, so that a position of any size
-// keeps its angle to 2^-24 of a turn; sine, cosine and the products are float32
-// and each result is rounded once.
+// float64 (three roundings, 3 x 2^-53 of it) and reduced to half a turn there, so
+// that it keeps 2^-24 of a turn up to 2^27 turns, 2^-23 at the ends of int32 with one
+// radian a position, and beyond what float64 holds; sine, cosine and the products
+// are float32 and each result is rounded once.
 //
 // Bound by memory: every element is read and written once.  A wave takes one
 // token: each of its 64 lanes forms the sine and cosine of one pair, once per
@@ -202,7 +203,7 @@ extern "C" int ssa_paged_append(const void* q, long long q_token_stride, long lo
       heads + 2ll * kv_heads > 65536 || pages <= 0 || table_pages <= 0 || (!starts && tokens % batch) || (flags & ~3))
     return (int)hipErrorInvalidValue;
   if (pairs < 0 || pairs > kHeadDim / 2 || (!interleaved && pairs % 8) || (pairs > 0 && !freqs) || axes < 1 ||
-      axes > 3 || axis0 < 0 || axis1 < 0 || axis0 > pairs - axis1 || (axes > 1 && !positions && pairs > 0))
+      axes > 3 || first > 1ll << 53 || first < -(1ll << 53) || axis0 < 0 || axis1 < 0 || axis0 > pairs - axis1 || (axes > 1 && !positions && pairs > 0))
     return (int)hipErrorInvalidValue;
   // pairs behind the counts turn on the next axis, which positions must hold
   if (positions && pairs > 0 && ((axes == 1 && axis0 != pairs) || (axes == 2 && axis0 + axis1 != pairs)))

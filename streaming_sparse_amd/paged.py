@@ -25,6 +25,7 @@ from .legacy_components import HEAD_DIM
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _INT, _F64 = torch.int32, torch.float64
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_FAR = 1 << 53                  # positions that float64 counts one by one
 _PARTS = {None: 0, True: 1 << 3, False: 2 << 3}        # single_av as the call's flags
 
 
@@ -135,7 +136,8 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
     with R a multiple of 8.  A token's position is first + held[b] + i, or
     given by `positions` int32 [N] or [N, A]: the first axes[0] pairs turn on
     the first axis, and so on (axes: up to 3 counts that sum to R).  Angles
-    are formed in float64.
+    are formed in float64: within 2^-24 of a turn up to 2^27 turns, and as
+    float64 holds them beyond; `first` lies within 2^53.
 
     q_out: where the rotated queries go (q itself is allowed; otherwise it must
     not overlap what is read); else a buffer owned by `workspace` that the next
@@ -145,6 +147,8 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
     code = _TYPES.get(dtype)
     if code is None:
         raise TypeError("k must be bfloat16 or float16")
+    if not -_FAR <= first <= _FAR:
+        raise ValueError("first must lie within 2^53")
     n, g, k_tok, k_head, k_ptr = _rows(k, "k", dtype, dev)
     nv, gv, v_tok, v_head, v_ptr = _rows(v, "v", dtype, dev)
     rows, gc, kv_tok, kv_head = _cache(cache_k, cache_v, dtype, dev)

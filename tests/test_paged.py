@@ -325,3 +325,19 @@ def test_attention_rejects_what_is_no_precision():
 def test_attention_abi_rejects_unknown_flags():
     for flags in (3 << 3, 1 << 5, 4 | 1 << 3, -1):
         assert attention_call(flags=flags) == INVALID, flags
+
+
+@built
+def test_append_rejects_a_first_position_that_float64_cannot_count(no_launch):
+    """Positions are counted in 64 bits and become float64: `first` beyond 2^53 would
+    be taken for another, or wrap."""
+    a = args()
+    for first in (2 ** 53 + 1, -2 ** 53 - 1, 2 ** 63, 2 ** 64 + 5):
+        with pytest.raises(ValueError):
+            paged.append(a['k'], a['v'], a['ck'], a['cv'], a['table'], a['held'], freqs=a['f'], first=first)
+    for first in (2 ** 53, -2 ** 53, 0):
+        paged.append(a['k'], a['v'], a['ck'], a['cv'], a['table'], a['held'], freqs=a['f'], first=first)
+    assert [given[21] for _, given in no_launch] == [2 ** 53, -2 ** 53, 0]
+    for first in (2 ** 53 + 1, -2 ** 53 - 1, 2 ** 63 - 1, -2 ** 63):
+        assert append_call(first=first) == INVALID
+    assert append_call(first=2 ** 53) == append_call(first=-2 ** 53) == 0
