@@ -36,10 +36,10 @@ extern "C" {
  * freqs[j] (float64, radians): elements (2j, 2j + 1) with flags bit 1, else (j,
  * j + pairs), pairs then a multiple of 8.  The position is first + at (first
  * within 2^53), or positions[t, axis] (int32 [tokens, axes], axes 1..3, wanted
- * for axes > 1): the first axis0 pairs turn on axis 0, the next axis1 on axis 1, the others on
- * axis 2; with positions the counts must reach the last of fewer axes: axis0 =
- * pairs for one, axis0 + axis1 = pairs for two.  Angles are formed in float64;
- * each result is rounded once.
+ * for axes > 1): the first axis0 pairs turn on axis 0, the next axis1 on axis 1,
+ * the others on axis 2; with positions the counts must reach the last of fewer
+ * axes: axis0 = pairs for one, axis0 + axis1 = pairs for two.  Angles are formed
+ * in float64; each result is rounded once.
  *
  * q [tokens, heads, 128] goes to q_out (which may be q itself); heads = 0: no
  * queries.  k and v must not overlap the cache rows written.  tokens is at most

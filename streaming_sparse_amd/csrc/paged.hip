@@ -1126,7 +1126,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedParams p) {
 struct Plan {
   int rows, row_tiles, prefix_tiles, prefix_pieces, prefix_cut, own_tiles, own_whole, own_pieces, own_cut;
   int own_groups, own_waves;     // apart: workgroups of own items, and their waves that take some
-  bool longest_first;
+  bool longest_first, pairs;     // pairs: wide tiles take two pages between barriers
   bool apart() const { return prefix_tiles > 0; }
   long long split_tiles(int kv_heads) const { return (long long)kv_heads * own_tiles - own_whole; }
   long long states(int kv_heads) const {
@@ -1237,6 +1237,7 @@ double plan_apart(const Sizes& z, Plan* plan) {
   plan->own_tiles = z.seq_tiles(kNarrow);
   plan->own_whole = 0;
   plan->longest_first = true;
+  plan->pairs = false;
   const double tiles = (double)z.kv_heads * plan->prefix_tiles, own_tiles = (double)z.kv_heads * plan->own_tiles;
   const double live = (double)rows / plan->prefix_tiles;
   const double floor_time = page_time(z.kv_heads * (prefix_pages + 0.6 * z.batch * z.table_pages));
@@ -1325,6 +1326,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
   const bool wide = T > kNarrow, singly = per_seq <= 192;       // pages one by one
   const int slots = wide ? z.cus : 2 * z.cus;
   plan->rows = T;
+  plan->pairs = wide && !singly;
   plan->row_tiles = plan->prefix_tiles = plan->prefix_pieces = plan->prefix_cut = 0;
   plan->own_groups = plan->own_waves = 0;
   plan->own_tiles = z.seq_tiles(T);
@@ -1495,7 +1497,6 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   auto start = [&](auto f16_kernel, auto bf16_kernel) {
     f16 ? launch(f16_kernel, items, 64 * waves) : launch(bf16_kernel, items, 64 * waves);
   };
-  const bool pairs = !plan.apart() && (long long)tokens * p.group / batch > 192;
   if (!wide && plan.apart())
     start(narrow_kernel<true, true>, narrow_kernel<false, true>);
   else if (!wide)
@@ -1503,7 +1504,7 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   else if (plan.apart())
     two ? start(wide_kernel<true, true, false, true>, wide_kernel<false, true, false, true>)
         : start(wide_kernel<true, true, false, false>, wide_kernel<false, true, false, false>);
-  else if (pairs)
+  else if (plan.pairs)
     two ? start(wide_kernel<true, false, true, true>, wide_kernel<false, false, true, true>)
         : start(wide_kernel<true, false, true, false>, wide_kernel<false, false, true, false>);
   else
