@@ -72,8 +72,9 @@ int ssa_paged_append(const void* q, long long q_token_stride, long long q_head_s
  *
  * A probability meets V in 16 bits, in two parts (hi + lo) or in one: flags bits
  * 3 and 4 are 1 for one part in all tiles of more than 32 query rows a K/V head,
- * 2 for two parts throughout, 0 for one only where the sequences bring more than
- * 32 rows (their mean) and walk the prefix in tiles of their own.  Bit 2 is 0.
+ * 2 for two parts throughout, 0 for one in those tiles where the sequences bring
+ * more than 32 rows (their mean, tokens / batch * heads / kv_heads), else two.
+ * Bit 2 is 0.
  *
  * workspace: 16-byte aligned, at least ssa_paged_attention_workspace_bytes of
  * the same sizes, any contents; calls that share one must not overlap. */

@@ -653,11 +653,11 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
 // 0.00235 relative, with two parts 0.00166; fp16 0.000286 and 0.000207).  The second
 // part is half as many products again: 4 x 4608 tokens behind 23040 rows 2686 and
 // 3722 us, 8 x 1536 behind 4608 422 and 573, six prompts of up to 901 behind 8192
-// 464 and 635.  So it is the caller's to ask for where a sequence fills tiles by
-// itself.  Tiles of a prefix apart hold the steps of many sequences, each of which
-// alone would take a narrow tile: they take two parts unless asked otherwise, so
-// that a step's precision does not change with the batch (64 x 1 behind 16384 48.3
-// and 51.4 us, 16 x 1 behind 131001 118.9 and 123.6, 24 x 5 behind 5003 27.9 and 32.1).
+// 464 and 635.  So it is the caller's to ask for, but for sequences of up to 32 rows
+// a K/V head (their mean), which alone would take narrow tiles: where they meet in
+// the tiles of a prefix apart they have two parts as well, so that a step's precision
+// does not change with the batch (64 x 1 behind 16384 48 and 51 us, 16 x 1 behind
+// 131001 118 and 121).
 // 4 sequences of 4608 tokens, 12 heads, behind 23040 rows: 2614 us, 1.20 PFLOP/s
 // (an 8192^3 library product 1.40), the matrix pipe busy 65% of the time and the
 // vector pipe 55 at the 1.65 GHz that the chip holds under this load.  Waves of 64
@@ -1160,7 +1160,7 @@ struct Plan {
 // page takes 0.93 to 0.98 us with up to 128 rows (a wave on each SIMD), 1.35 with
 // 192, with 256 1.62 where all CUs work and 1.32 where few do (the clock falls
 // under the matrix pipe's load), 7% less with two pages between barriers; in two
-// parts (a prefix apart) 1.15 to 2.0 (64 x 1 token behind 16384 cut by the figures of
+// parts (steps behind a prefix apart) 1.15 to 2.0 (64 x 1 token behind 16384 cut by the figures of
 // one part 55.9 us, by these 51.4; 128 x 1 behind 4096 69.3 and 58.4); a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A page that no other tile reads
 // takes 1.1 and 1.2 at least, which is what one workgroup draws from memory.
 // Waves by themselves: a CU draws a page in 0.85 us (8 of them one each in 6.8), a
@@ -1213,6 +1213,7 @@ struct Sizes {
   }
   int prefix_pages() const { return (prefix_tokens + kPage - 1) / kPage; }
   long long rows() const { return (long long)tokens * (heads / kv_heads); }     // of a K/V head
+  bool few() const { return rows() <= (long long)kNarrow * batch; }    // a sequence fills no wide tile
   // tiles of T rows of a K/V head, of sequences by themselves, at most
   int seq_tiles(int T) const {
     return (int)(ragged ? rows() / T + batch : batch * ((rows() / batch + T - 1) / T));
@@ -1273,7 +1274,7 @@ double plan_apart(const Sizes& z, Plan* plan) {
     const int pieces = cut_in(prefix_pages, c, &cut);
     const double t = start_time(T, live, true) + cut * tile_page(T, std::min<double>(rows, T),
                                                            std::min(tiles * pieces, (double)slots), z.cus,
-                                                           plan->prefix_tiles == 1 ? 1.0 : 0.0, true, true);
+                                                           plan->prefix_tiles == 1 ? 1.0 : 0.0, true, z.few());
     const double rounds = std::ceil(tiles * pieces / slots), left = rounds * slots - tiles * pieces;
     for (int d : kCuts) {
       if (d > 16 || (d > 1 && 2 * d > z.table_pages)) break;
@@ -1386,15 +1387,14 @@ int make_plan(Sizes z, Plan* plan) {
   static thread_local Plan last_plan;
   if (!(z == last_sizes)) {
     Plan joint, other;
-    const bool narrow = z.rows() <= (long long)kNarrow * z.batch;
-    double t = plan_joint(z, narrow ? kNarrow : kWide, &joint);
+    double t = plan_joint(z, z.few() ? kNarrow : kWide, &joint);
     auto consider = [&](double time) {
       if (time < t) {
         joint = other;
         t = time;
       }
     };
-    if (!narrow) consider(plan_joint(z, kHalfWide, &other));
+    if (!z.few()) consider(plan_joint(z, kHalfWide, &other));
     if (z.batch > 1 && z.prefix_tokens > 0) consider(plan_apart(z, &other));
     last_plan = joint;
     last_sizes = z;
@@ -1436,8 +1436,9 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
       (((uintptr_t)q | (uintptr_t)cache_k | (uintptr_t)cache_v | (uintptr_t)out) & 15) || ((uintptr_t)lse & 3))
     return (int)hipErrorInvalidValue;
   Plan plan;
-  const int e = make_plan(Sizes{0, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr,
-                                (flags & 2) != 0}, &plan);
+  const Sizes sizes{0, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr,
+                    (flags & 2) != 0};
+  const int e = make_plan(sizes, &plan);
   if (e != (int)hipSuccess) return e;
   if (!plan.fits(kv_heads)) return (int)hipErrorInvalidValue;
   const long long need = plan.bytes(kv_heads);
@@ -1488,9 +1489,9 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
   const int waves = plan.waves();
   const bool wide = plan.wide(), many = plan.many();
   const bool f16 = flags & 1;
-  // parts of a probability in wide tiles: as asked, else two with the prefix apart
+  // parts of a probability in wide tiles: as asked, else two for sequences of few rows
   const int parts = flags >> 3;
-  const bool two = parts ? parts == 2 : plan.apart();
+  const bool two = parts ? parts == 2 : sizes.few();
   auto launch = [&](auto kernel, long long blocks, int threads) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, p);
   };

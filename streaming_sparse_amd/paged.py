@@ -238,10 +238,10 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     probability meets V in 16 bits (fp16: scaled up by 2^7): in two parts (hi
     + lo), which leave the output its own rounding, or in one, with which its
     error is 1.4 times as large.  ``single_av=False``: two parts throughout;
-    the default None: two, but one where the sequences bring more than 32 rows
-    a K/V head (their mean) and walk the prefix in tiles of their own, which
-    the matrix pipe bounds (two parts take 1.4 times as long there);
-    ``single_av=True``: one in all tiles of more than 32 rows.  Sums reach 2^8 times the values' size times the rows: bf16
+    the default None: two where the sequences bring up to 32 rows a K/V head
+    (their mean: new tokens times H / G), else one in tiles of more than 32
+    rows, which the matrix pipe bounds (two parts take 1.4 times as long
+    there); ``single_av=True``: one in all tiles of more than 32 rows.  Sums reach 2^8 times the values' size times the rows: bf16
     values from 2^96 on, and fp16 values within 2^-11 of the type's largest,
     may come out infinite."""
     device, dtype, dev = q.device, q.dtype, q.get_device()

@@ -26,6 +26,7 @@ CASES = [
     pytest.param(90, 1, True, 700, 6, 2, 20000, True, BF16, 2, id='apart_wide_many_pieces'),
     pytest.param(64, 1, True, 600, 16, 4, 16384, True, FP16, 2, id='apart_wide_steps'),
     pytest.param(30, 7, True, 90, 14, 2, 700, True, FP16, 1, id='joint_wide_few_tokens'),
+    pytest.param(24, 5, True, 333, 28, 4, 5003, True, FP16, 1, id='apart_wide_more_rows'),
     pytest.param(300, 1, True, 130, 16, 8, 700, True, BF16, 2, id='apart_items_in_turn'),
     pytest.param(1, 200, True, 50, 8, 2, 30000, True, BF16, 1, id='joint_wide_many_pieces'),
     pytest.param(20, 64, True, 900, 12, 12, 0, True, FP16, 1, id='joint_wide_few_rows'),
