@@ -658,9 +658,9 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void narrow_kernel(PagedParam
 // the tiles of a prefix apart they have two parts as well, so that a step's precision
 // does not change with the batch (64 x 1 behind 16384 48 and 51 us, 16 x 1 behind
 // 131001 118 and 121).
-// 4 sequences of 4608 tokens, 12 heads, behind 23040 rows: 2614 us, 1.20 PFLOP/s
-// (an 8192^3 library product 1.40), the matrix pipe busy 65% of the time and the
-// vector pipe 55 at the 1.65 GHz that the chip holds under this load.  Waves of 64
+// 4 sequences of 4608 tokens, 12 heads, behind 23040 rows: 2649 us, 1.18 PFLOP/s
+// (an 8192^3 library product 1.40), the matrix pipe busy 64% of the time and the
+// vector pipe 56 at the 1.65 GHz that the chip holds under this load.  Waves of 64
 // rows, one on a SIMD, read half as much LDS and took 2948 us where these took 2711;
 // from there the slots at fixed offsets, the raised priority and the loads between
 // the half pages.  The sums as dot products of the rounded pairs, half as many
@@ -1121,8 +1121,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedParams p) {
   if (p.lse && dims == 0) p.lse[(long long)token * p.heads + hq] = lse_of(M, L);
 }
 
-// How a call is cut up, from sizes alone.  Tiles are of 32 rows (narrow) or 256
-// (wide); own tiles beside prefix tiles are narrow.
+// How a call is cut up, from sizes alone.  Tiles are of 32 rows (narrow), or of 256
+// or, in one list, 128 (wide); own tiles beside prefix tiles are narrow.
 struct Plan {
   int rows, row_tiles, prefix_tiles, prefix_pieces, prefix_cut, own_tiles, own_whole, own_pieces, own_cut;
   int own_groups, own_waves;     // apart: workgroups of own items, and their waves that take some
@@ -1164,8 +1164,12 @@ struct Plan {
 // one part 55.9 us, by these 51.4; 128 x 1 behind 4096 69.3 and 58.4); a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A page that no other tile reads
 // takes 1.1 and 1.2 at least, which is what one workgroup draws from memory.
 // Waves by themselves: a CU draws a page in 0.85 us (8 of them one each in 6.8), a
-// wave one in 3.5, and an item begins and ends in 5. Tables are taken to be 0.6 to
-// 0.7 full, which only shifts the choice.
+// wave one in 3.5, and an item begins and ends in 5.  The lengths being known to the
+// device alone, tables are taken to be 0.6 to 0.7 full and sequences to be of mean
+// size.  In a table much wider than its sequences the own pages seem to cover for a
+// longer walk of the prefix, which is then cut too little (64 x 1 token behind 16384,
+// up to 600 rows of their own: 51 us with a table of 10 pages, 69 with 32, 123 with 64,
+// 460 with 256; 16 x 1 behind 131001 128 us with 33 pages, 211 with 256).
 constexpr double kJoinStart = 3.0, kSoloPage = 0.85, kSoloLatency = 3.5, kSoloStart = 3.0, kSoloItem = 5.0;
 double start_time(int T, double rows, bool singly) {
   return T == kNarrow ? 7.0 : singly ? 6.0 + 5.0 * rows / kWide : 5.0 + 3.0 * rows / kWide;
@@ -1222,7 +1226,7 @@ struct Sizes {
 
 // The prefix apart: all rows together over the prefix, each sequence over its own
 // pages.  Returns the estimated time.  Against one list, us: 64 x 1 token, 32 heads on
-// 8, behind 16384: 48 and 228; 16 x 1 behind 131001: 118 and 1089; 24 x 5, 28 on 4,
+// 8, behind 16384: 51 and 228; 16 x 1 behind 131001: 121 and 1089; 24 x 5, 28 on 4,
 // behind 5003: 27 and 54; where sequences fill tiles, 8 x 1536 behind 4608, 579 and
 // 422.  The own lists' first pieces come first, then the second ones, on the CUs the
 // prefix leaves (64 x 1 behind 2048, up to 2000 own rows: 75, list by list 85), as

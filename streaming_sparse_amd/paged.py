@@ -11,7 +11,10 @@ b's at rows starts[b] .. starts[b + 1] - 1 of [N, heads, 128] tensors (starts
 
 Every size on the host is a bound only: how many tokens a sequence holds and
 where its rows start are read on the device, so a captured call is replayed
-with other values.  Nothing here computes on the CPU.
+with other values.  The attention's work is cut up by those bounds, though: a
+table much wider than the sequences are long costs time (64 sequences of up to
+600 rows behind 16384: 51 us with 10 pages a row, 123 with 64, 460 with 256).
+Nothing here computes on the CPU.
 """
 from __future__ import annotations
 
