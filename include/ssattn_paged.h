@@ -68,7 +68,8 @@ int ssa_paged_append(const void* q, long long q_token_stride, long long q_head_s
  * place change.  Values in
  * rows of a page that no query sees (behind a sequence's or the prefix's end)
  * may be anything, NaN included; one that some query of the call sees must be
- * finite for the others to come out finite.  out may be q itself.
+ * finite for the others to come out finite (an infinite one may come out NaN).
+ * out may be q itself.
  *
  * A probability meets V in 16 bits, in two parts (hi + lo) or in one: flags bits
  * 3 and 4 are 1 for one part in all tiles of more than 32 query rows a K/V head,
@@ -86,7 +87,8 @@ int ssa_paged_attention(const void* q, long long q_token_stride, long long q_hea
                         float scale, int flags, void* workspace, long long workspace_bytes, hipStream_t stream);
 
 /* Bytes of that workspace (0: none needed), from sizes alone; -1 for sizes the
- * call rejects (tokens * heads >= 2^30, or more work than a grid holds).  ragged: whether the call gives starts; causal: whether it is. */
+ * call rejects (tokens * heads >= 2^30, or more work than a grid holds).
+ * ragged: whether the call gives starts; causal: whether it is. */
 long long ssa_paged_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int prefix_tokens,
                                               int table_pages, int ragged, int causal);
 

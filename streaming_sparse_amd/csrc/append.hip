@@ -203,8 +203,10 @@ extern "C" int ssa_paged_append(const void* q, long long q_token_stride, long lo
       heads + 2ll * kv_heads > 65536 || pages <= 0 || table_pages <= 0 || (!starts && tokens % batch) || (flags & ~3))
     return (int)hipErrorInvalidValue;
   if (pairs < 0 || pairs > kHeadDim / 2 || (!interleaved && pairs % 8) || (pairs > 0 && !freqs) || axes < 1 ||
-      axes > 3 || first > 1ll << 53 || first < -(1ll << 53) || axis0 < 0 || axis1 < 0 || axis0 > pairs - axis1 || (axes > 1 && !positions && pairs > 0))
+      axes > 3 || axis0 < 0 || axis1 < 0 || axis0 > pairs - axis1 || (axes > 1 && !positions && pairs > 0))
     return (int)hipErrorInvalidValue;
+  // beyond, float64 does not hold every position
+  if (first > 1ll << 53 || first < -(1ll << 53)) return (int)hipErrorInvalidValue;
   // pairs behind the counts turn on the next axis, which positions must hold
   if (positions && pairs > 0 && ((axes == 1 && axis0 != pairs) || (axes == 2 && axis0 + axis1 != pairs)))
     return (int)hipErrorInvalidValue;

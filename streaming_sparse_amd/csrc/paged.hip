@@ -1160,9 +1160,10 @@ struct Plan {
 // page takes 0.93 to 0.98 us with up to 128 rows (a wave on each SIMD), 1.35 with
 // 192, with 256 1.62 where all CUs work and 1.32 where few do (the clock falls
 // under the matrix pipe's load), 7% less with two pages between barriers; in two
-// parts (steps behind a prefix apart) 1.15 to 2.0 (64 x 1 token behind 16384 cut by the figures of
-// one part 55.9 us, by these 51.4; 128 x 1 behind 4096 69.3 and 58.4); a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A page that no other tile reads
-// takes 1.1 and 1.2 at least, which is what one workgroup draws from memory.
+// parts (steps behind a prefix apart) 1.15 to 2.0 (64 x 1 token behind 16384 cut by
+// the figures of one part 55.9 us, by these 51.4; 128 x 1 behind 4096 69.3 and 58.4);
+// a narrow tile's 0.47, 0.72 with two workgroups on a CU.  A page that no other tile
+// reads takes 1.1 and 1.2 at least, which is what one workgroup draws from memory.
 // Waves by themselves: a CU draws a page in 0.85 us (8 of them one each in 6.8), a
 // wave one in 3.5, and an item begins and ends in 5.  The lengths being known to the
 // device alone, tables are taken to be 0.6 to 0.7 full and sequences to be of mean
@@ -1174,7 +1175,7 @@ constexpr double kJoinStart = 3.0, kSoloPage = 0.85, kSoloLatency = 3.5, kSoloSt
 double start_time(int T, double rows, bool singly) {
   return T == kNarrow ? 7.0 : singly ? 6.0 + 5.0 * rows / kWide : 5.0 + 3.0 * rows / kWide;
 }
-double tile_page(int T, double rows, double active, double cus, double unshared, bool singly, bool two) {
+double tile_page(int T, double rows, double active, double cus, double unshared, bool singly, bool two = false) {
   const double busy = active / cus;
   double page;
   if (T == kNarrow) {
@@ -1359,7 +1360,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
     double time, states = 0.0;
     if (plan->longest_first) {
       const double mean = units - 0.5 * spread, each = std::max(1.0, mean / cut + (c > 1 ? 0.5 : 0.0));
-      const double page = tile_page(T, full, std::min(tiles * each, (double)slots), z.cus, unshared, singly, false);
+      const double page = tile_page(T, full, std::min(tiles * each, (double)slots), z.cus, unshared, singly);
       const double longest = start + cut * page;
       time = tiles * each <= slots ? longest
                                    : std::max(longest, tiles * (each * start + mean * page) / slots + 0.5 * longest);
@@ -1367,7 +1368,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
     } else {
       const double active = std::min(tiles * pieces, (double)slots);
       time = std::ceil(tiles * pieces / slots) *
-             (start + std::max(cut * tile_page(T, full, active, z.cus, unshared, singly, false),
+             (start + std::max(cut * tile_page(T, full, active, z.cus, unshared, singly),
                                page_time(read * active * cut, active / z.cus)));
       states = pieces > 1 ? tiles * pieces : 0.0;
     }
@@ -1379,7 +1380,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
     }
   }
   plan->own_whole = (int)(plan->own_pieces == 1 ? own_tiles : whole);
-  return least + (double)(whole / z.cus) * (start + units * tile_page(T, full, slots, z.cus, unshared, singly, false));
+  return least + (double)(whole / z.cus) * (start + units * tile_page(T, full, slots, z.cus, unshared, singly));
 }
 
 // The plan of a call's sizes (z.cus is filled in).  A thread keeps its last one:

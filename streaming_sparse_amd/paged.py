@@ -229,7 +229,7 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     as they were.  Pages outside the cache (-1) and, where a length passes it,
     behind the table's end count as absent; rows that no query sees may hold
     anything, while a value row that some query of the call sees must be
-    finite for the others to come out finite.
+    finite for the others to come out finite (an infinite one may come out NaN).
 
     scale defaults to 128 ** -0.5.  Returns out [N, H, 128], or (out, lse)
     with want_lse, lse [N, H] float32 the log of the sum of exponentials:
@@ -244,9 +244,9 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     the default None: two where the sequences bring up to 32 rows a K/V head
     (their mean: new tokens times H / G), else one in tiles of more than 32
     rows, which the matrix pipe bounds (two parts take 1.4 times as long
-    there); ``single_av=True``: one in all tiles of more than 32 rows.  Sums reach 2^8 times the values' size times the rows: bf16
-    values from 2^96 on, and fp16 values within 2^-11 of the type's largest,
-    may come out infinite."""
+    there); ``single_av=True``: one in all tiles of more than 32 rows.  Sums
+    reach 2^8 times the values' size times the rows: bf16 values from 2^96 on,
+    and fp16 values within 2^-11 of the type's largest, may come out infinite."""
     device, dtype, dev = q.device, q.dtype, q.get_device()
     code = _TYPES.get(dtype)
     if code is None:
