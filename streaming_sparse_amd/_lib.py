@@ -1,5 +1,5 @@
-"""ctypes binding of libssattn.so (declared in include/ssattn.h and
-include/ssattn_paged.h).
+"""ctypes binding of libssattn.so (declared in include/ssattn.h,
+include/ssattn_paged.h and include/ssattn_paged8.h).
 
 The library is built in-tree by ``streaming_sparse_amd.build``.  There is no
 fallback: if the library is missing or a call fails, an error is raised.
@@ -18,7 +18,8 @@ _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or \
 
 _vp, _i, _ll, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 # return type of the entry points that do not return a status
-RESTYPES = {"ssa_attention_workspace_bytes": _ll, "ssa_paged_attention_workspace_bytes": _ll}
+RESTYPES = {"ssa_attention_workspace_bytes": _ll, "ssa_paged_attention_workspace_bytes": _ll,
+            "ssa_paged8_workspace_bytes": _ll}
 SIGNATURES = {
     "ssa_route_stamps": [_vp, _ll],
     "ssa_attn_stamps": [_vp, _ll],
@@ -49,6 +50,17 @@ SIGNATURES = {
     "ssa_paged_attention": [_vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _i, _vp, _vp, _vp, _vp, _ll, _ll, _vp, _i, _i, _i,
                             _i, _i, _i, _f, _i, _vp, _ll, _vp],
     "ssa_paged_attention_workspace_bytes": [_i, _i, _i, _i, _i, _i, _i, _i],
+    "ssa_paged_attention_shaped": [_vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _i, _vp, _vp, _vp, _vp, _ll, _ll, _vp, _i, _i,
+                                   _i, _i, _i, _i, _f, _f, _vp, _i, _i, _vp, _ll, _vp],
+    "ssa_paged8_append": [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _ll, _ll,
+                          _vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "ssa_paged8_read": [_vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _i, _i, _i, _i,
+                        _i, _i, _vp],
+    "ssa_paged8_attention": [_vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _vp, _vp, _vp, _vp, _ll, _ll,
+                             _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _ll, _vp],
+    "ssa_paged8_attention_shaped": [_vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _vp, _vp, _vp, _vp, _ll,
+                                    _ll, _vp, _i, _i, _i, _i, _i, _i, _f, _f, _vp, _i, _i, _vp, _ll, _vp],
+    "ssa_paged8_workspace_bytes": [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i],
     "ssa_pset_noalloc": [_vp, _ll, _ll, _ll, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i,
                          _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
 }

@@ -19,7 +19,8 @@ LIB = os.path.join(HERE, "libssattn.so")
 # measurement build: the same sources with the router's phase stamps and the
 # attention kernel's step stamps compiled in
 STAMPS_LIB = os.path.join(HERE, "libssattn_stamps.so")
-SOURCES = ("attention.hip", "route.hip", "pset.hip", "summary.hip", "runtime.hip", "group.hip", "append.hip", "paged.hip")
+SOURCES = ("attention.hip", "route.hip", "pset.hip", "summary.hip", "runtime.hip", "group.hip", "append.hip", "paged.hip",
+           "paged_shaped.hip", "paged8.hip", "paged8_shaped.hip")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
          # packed fp32 VALU forms are excluded from code generation
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -35,6 +35,24 @@ __device__ __forceinline__ u32x4 ldg16(const uint16_t* p) {
   return *reinterpret_cast<const u32x4*>(p);
 }
 
+// Eight 8-bit values times a power of two (a float's exponent) as 16-bit ones, exactly.
+template <bool F16>
+__device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi, float scale) {
+  u32x4 r;
+  if constexpr (F16) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, scale, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, scale, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, scale, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, scale, true));
+  } else {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, scale, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, scale, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, scale, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, scale, true));
+  }
+  return r;
+}
+
 // D[32x32] += A[32x16] * B[16x32], bf16 inputs, fp32 accumulate.
 // Lane l: A row l%32, k = 8*(l/32)+i; B col l%32, same k; D col l%32,
 // rows 8*(i/4) + 4*(l/32) + i%4 for accumulator item i.
@@ -96,25 +114,29 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t l
 
 // N consecutive 1 KB global->LDS loads of one wave: load jj reads base +
 // off[jj] + jj * 1024 (per lane) into lds + jj * 1024 + 16 * lane, with one
-// M0 value for all of them.
-template <int N>
+// M0 value for all of them.  NOP + 1 wait states come first: an address in
+// scalar registers that a vector instruction has written (a readfirstlane, a
+// spilled register's reload) needs five before a load reads it, which the
+// compiler does not see to in inline asm; one that scalar instructions form
+// needs none.
+template <int N, int NOP = 0>
 __device__ __forceinline__ void dma_rows(const void* base, const uint32_t (&off)[4], uint32_t lds) {
   if constexpr (N == 4) {
     asm volatile(
-        "s_nop 0\n\t"
+        "s_nop %6\n\t"
         "global_load_lds_dwordx4 %0, %4\n\t"
         "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
         "global_load_lds_dwordx4 %2, %4 offset:2048\n\t"
         "global_load_lds_dwordx4 %3, %4 offset:3072" ::"v"(off[0]),
-        "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "{m0}"(lds)
+        "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "{m0}"(lds), "n"(NOP)
         : "memory");
   } else {
     static_assert(N == 2, "2 or 4 loads");
     asm volatile(
-        "s_nop 0\n\t"
+        "s_nop %4\n\t"
         "global_load_lds_dwordx4 %0, %2\n\t"
         "global_load_lds_dwordx4 %1, %2 offset:1024" ::"v"(off[0]),
-        "v"(off[1]), "s"(base), "{m0}"(lds)
+        "v"(off[1]), "s"(base), "{m0}"(lds), "n"(NOP)
         : "memory");
   }
 }

@@ -29,18 +29,19 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _INT, _F64 = torch.int32, torch.float64
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
 _FAR = 1 << 53                  # positions that float64 counts one by one
+_MOST_ROWS = (1 << 30) - 1      # of a sequence, and of a window
 _PARTS = {None: 0, True: 1 << 3, False: 2 << 3}        # single_av as the call's flags
 
 
 # The checks below stand in the path of a call of a few microseconds, so each
 # property of a tensor is asked for once and devices are compared by index.
 
-def _overlap(rows, heads, tok, head):
-    """Whether rows of 128 elements at r * tok + h * head may share elements:
+def _overlap(rows, heads, tok, head, size=HEAD_DIM):
+    """Whether rows of `size` elements at r * tok + h * head may share elements:
     neither do the heads of a token lie between two tokens, nor the tokens of
     a head between two heads."""
-    return (tok < (heads - 1) * head + HEAD_DIM and rows > 1 or head < HEAD_DIM and heads > 1) and \
-        (head < (rows - 1) * tok + HEAD_DIM and heads > 1 or tok < HEAD_DIM and rows > 1)
+    return (tok < (heads - 1) * head + size and rows > 1 or head < size and heads > 1) and \
+        (head < (rows - 1) * tok + size and heads > 1 or tok < size and rows > 1)
 
 
 def _cache(cache_k, cache_v, dtype, dev):
@@ -152,9 +153,17 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
         raise TypeError("k must be bfloat16 or float16")
     if not -_FAR <= first <= _FAR:
         raise ValueError("first must lie within 2^53")
+    rows, g, kv_tok, kv_head = _cache(cache_k, cache_v, dtype, dev)
+    return _append("ssa_paged_append", (cache_k.data_ptr(), cache_v.data_ptr(), kv_tok, kv_head), rows >> 6, g, k, v,
+                   table, held, q, q_out, starts, freqs, axes, positions, first, interleaved, workspace, code)
+
+
+def _append(entry, cache, pages, gc, k, v, table, held, q, q_out, starts, freqs, axes, positions, first, interleaved,
+            workspace, code):
+    """append to the cache that the entry takes as `cache`."""
+    device, dtype, dev = k.device, k.dtype, k.get_device()
     n, g, k_tok, k_head, k_ptr = _rows(k, "k", dtype, dev)
     nv, gv, v_tok, v_head, v_ptr = _rows(v, "v", dtype, dev)
-    rows, gc, kv_tok, kv_head = _cache(cache_k, cache_v, dtype, dev)
     if nv != n or gv != g or gc != g:
         raise ValueError("k and v must be [N, G, 128] for the cache's G heads")
     batch, width, table_ptr, starts_ptr = _sequences(table, starts, n, dev)
@@ -201,10 +210,9 @@ def append(k, v, cache_k, cache_v, table, held, *, q=None, q_out=None, starts=No
     elif q_out is not None:
         raise ValueError("q_out without q")
     if n:
-        _launch("ssa_paged_append", device, dev, q_ptr, q_tok, q_head, out_ptr, o_tok, o_head, k_ptr, k_tok, k_head,
-                v_ptr, v_tok, v_head, cache_k.data_ptr(), cache_v.data_ptr(), kv_tok, kv_head, table_ptr, held_ptr,
-                starts_ptr, pos_ptr, freqs_ptr, first, n, batch, h, g, rows >> 6, width, pairs, a0, a1, na,
-                code | 2 if interleaved else code)
+        _launch(entry, device, dev, q_ptr, q_tok, q_head, out_ptr, o_tok, o_head, k_ptr, k_tok, k_head, v_ptr, v_tok,
+                v_head, *cache, table_ptr, held_ptr, starts_ptr, pos_ptr, freqs_ptr, first, n, batch, h, g, pages,
+                width, pairs, a0, a1, na, code | 2 if interleaved else code)
     return q_out
 
 
@@ -214,7 +222,7 @@ _BYTES = {}
 
 
 def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, workspace, *, starts=None, causal=True,
-              scale=None, want_lse=False, out=None, single_av=None):
+              scale=None, want_lse=False, out=None, single_av=None, cap=None, slopes=None, window=None):
     """Attention of every sequence's new queries over the shared prefix and the
     sequence's own rows; the prefix is read for all sequences together.
 
@@ -246,13 +254,50 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     rows, which the matrix pipe bounds (two parts take 1.4 times as long
     there); ``single_av=True``: one in all tiles of more than 32 rows.  Sums
     reach 2^8 times the values' size times the rows: bf16 values from 2^96 on,
-    and fp16 values within 2^-11 of the type's largest, may come out infinite."""
-    device, dtype, dev = q.device, q.dtype, q.get_device()
-    code = _TYPES.get(dtype)
+    and fp16 values within 2^-11 of the type's largest, may come out infinite.
+
+    Shaped scores, each for itself or together, of s = scale q.k:
+    cap (positive): s becomes cap tanh(s / cap), within 2^-22 of the cap;
+    slopes [H] float32: s falls by the head's slope times the distance in rows
+    between query and key, query i's own row being lengths[b] - n + i and the
+    prefix's rows lying before row 0 (keys behind the query count alike);
+    window (1 or more): of its own sequence a query sees only the `window` rows up
+    to its own (without `causal` also those behind it), and all of the prefix.
+    Pages that no query sees any more may be absent, and are not walked."""
+    code = _TYPES.get(q.dtype)
     if code is None:
         raise TypeError("q must be bfloat16 or float16")
+    dev = q.get_device()
+    rows, g, kv_tok, kv_head = _cache(cache_k, cache_v, q.dtype, dev)
+    return _attend("ssa_paged_attention", False, (cache_k.data_ptr(), cache_v.data_ptr(), kv_tok, kv_head), rows >> 6,
+                   g, q, prefix, prefix_tokens, table, lengths, workspace, starts, causal, scale, want_lse, out,
+                   single_av, cap, slopes, window, code)
+
+
+def _shape(cap, slopes, window, heads, dev):
+    """The entries' cap, slopes and window."""
+    if cap is None:
+        cap = 0.0
+    elif not 0.0 < cap < math.inf:
+        raise ValueError("cap must be positive")
+    slopes_ptr = None
+    if slopes is not None:
+        if slopes.dtype is not torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous() or \
+                slopes.get_device() != dev:
+            raise ValueError("slopes must be a contiguous float32 [H] tensor on the rows' device")
+        slopes_ptr = slopes.data_ptr()
+    if window is None:
+        window = 0
+    elif window < 1 or window != int(window):
+        raise ValueError("window must be a whole number from 1 on")
+    return cap, slopes_ptr, min(int(window), _MOST_ROWS)
+
+
+def _attend(entry, eight, cache, pages, g, q, prefix, prefix_tokens, table, lengths, workspace, starts, causal, scale,
+            want_lse, out, single_av, cap, slopes, window, code):
+    """attention over the cache that the entry takes as `cache`."""
+    device, dtype, dev = q.device, q.dtype, q.get_device()
     n, h, q_tok, q_head, q_ptr = _rows(q, "q", dtype, dev)
-    rows, g, kv_tok, kv_head = _cache(cache_k, cache_v, dtype, dev)
     if h == 0 or h % g:
         raise ValueError("the query heads must be a multiple of the cache's heads")
     batch, width, table_ptr, starts_ptr = _sequences(table, starts, n, dev)
@@ -283,15 +328,20 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     lse = lse_ptr = None
     if want_lse:
         lse, lse_ptr, _ = workspace.rows('paged_lse', (n, h), device, torch.float32)
+    shape = ()
+    if cap is not None or slopes is not None or window is not None:
+        shape = _shape(cap, slopes, window, h, dev)
+        entry += "_shaped"
     if n:
         key = (n, batch, h, g, prefix_tokens, width, starts is None, causal, dev)
+        if eight or shape:
+            key += (eight, bool(shape), shape[2] if shape else 0)
         need = _BYTES.get(key)
         if need is None:
             need = _workspace_bytes(key, device)
         part = workspace.tensor('paged_part', (need,), device, torch.uint8).data_ptr() if need else None
-        _launch("ssa_paged_attention", device, dev, q_ptr, q_tok, q_head, cache_k.data_ptr(), cache_v.data_ptr(),
-                kv_tok, kv_head, prefix_ptr, prefix_tokens, table_ptr, len_ptr, starts_ptr, out_ptr, o_tok, o_head,
-                lse_ptr, n, batch, h, g, rows >> 6, width, scale,
+        _launch(entry, device, dev, q_ptr, q_tok, q_head, *cache, prefix_ptr, prefix_tokens, table_ptr, len_ptr,
+                starts_ptr, out_ptr, o_tok, o_head, lse_ptr, n, batch, h, g, pages, width, scale, *shape,
                 (code | 2 if causal else code) | parts, part, need)
     return (out, lse) if want_lse else out
 
@@ -299,12 +349,13 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
 def _workspace_bytes(key, device):
     """The workspace of a call of these sizes, asked of the library once per sizes
     and device."""
-    tokens, batch, heads, kv_heads, prefix_tokens, width, equal, causal, dev = key
+    tokens, batch, heads, kv_heads, prefix_tokens, width, equal, causal, dev, *form = key
     if dev < 0:
         raise RuntimeError("the tensors must be on a GPU")
+    eight, shaped, window = form or (False, False, 0)
     with torch.cuda.device(device):
-        need = _lib.lib().ssa_paged_attention_workspace_bytes(tokens, batch, heads, kv_heads, prefix_tokens, width,
-                                                              int(not equal), int(bool(causal)))
+        need = _lib.lib().ssa_paged8_workspace_bytes(tokens, batch, heads, kv_heads, prefix_tokens, width,
+                                                     int(not equal), int(bool(causal)), int(eight), int(shaped), window)
     if need < 0:
         raise ValueError("paged.attention: sizes out of range")
     if need:
