@@ -75,6 +75,29 @@ __device__ __forceinline__ float from_lane(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_ds_bpermute(lane << 2, __float_as_int(x)));
 }
 
+__device__ __forceinline__ double from_lane(double x, int lane) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane << 2, (int)(uint32_t)u);
+  const uint32_t hi = __builtin_amdgcn_ds_bpermute(lane << 2, (int)(uint32_t)(u >> 32));
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+
+// Sine and cosine of h half turns, |h| <= 1, to 2^-45: their series about the nearest
+// quarter turn.
+__device__ __forceinline__ void turn64(double h, double* sine, double* cosine) {
+  const double quarter = __builtin_rint(2.0 * h), x = (h - 0.5 * quarter) * 3.141592653589793, t = x * x;
+  const double s =
+      x * (1 + t * (-1.0 / 6 + t * (1.0 / 120 + t * (-1.0 / 5040 + t * (1.0 / 362880 + t * (-1.0 / 39916800 +
+                                                                                        t * (1.0 / 6227020800)))))));
+  const double c =
+      1 + t * (-1.0 / 2 + t * (1.0 / 24 + t * (-1.0 / 720 + t * (1.0 / 40320 + t * (-1.0 / 3628800 +
+                                                                               t * (1.0 / 479001600 - t * (1.0 / 87178291200)))))));
+  const int q = (int)quarter;
+  const double a = q & 1 ? c : s, b = q & 1 ? s : c;
+  *sine = q & 2 ? -a : a;
+  *cosine = (q + 1) & 2 ? -b : b;
+}
+
 // The sequence and place of packed token t among sequences that start at starts[0..] (null:
 // per_seq tokens each); false: behind the last one.
 __device__ __forceinline__ bool place_of(const int32_t* starts, int batch, int per_seq, int t, int lane, int* b,
@@ -161,8 +184,15 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(AppendParams p) {
   if (!place_of(p.starts, p.batch, p.per_seq, t, lane, &b, &i)) return;      // a row behind the last sequence
   const long long at = (long long)p.held[b] + i;
   const long long row = cache_row(p.table, p.table_pages, p.pages, b, at);
+  // whether this wave's rows hold keys (EIGHT)
+  bool has_keys = false;
+  if constexpr (EIGHT) {
+    for (int r0 = slice * kRowsPerWave; r0 < p.heads + p.kv_heads; r0 += kRowsPerWave * p.slices)
+      has_keys |= r0 + kRowsPerWave > p.heads;
+  }
   // lane j's pair
   float cs = 1.0f, sn = 0.0f;
+  double cs64 = 1.0, sn64 = 0.0;
   if (lane < p.pairs) {
     double pos;
     if (p.positions) {
@@ -172,8 +202,11 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(AppendParams p) {
       pos = (double)(at + p.first);
     }
     const double turns = pos * (p.freqs[lane] * 0.15915494309189535);   // 1 / (2 pi)
-    const float half_turns = (float)(2.0 * (turns - __builtin_rint(turns)));
-    sincospif(half_turns, &sn, &cs);
+    const double half_turns = 2.0 * (turns - __builtin_rint(turns));
+    if (EIGHT && has_keys)
+      turn64(half_turns, &sn64, &cs64);
+    else
+      sincospif((float)half_turns, &sn, &cs);
   }
   const int c = lane & 15, sub = lane >> 4;
   constexpr int kNeed = INTERLEAVED ? 4 : 8;
@@ -183,12 +216,27 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(AppendParams p) {
   const bool second = !INTERLEAVED && c >= half_lanes;
   const int pair0 = INTERLEAVED ? 4 * c : 8 * (second ? c - half_lanes : c);
   const int partner = (lane & 48) | ((second ? c - half_lanes : c + half_lanes) & 15);
+  // 8-bit keys turn in float64: a step of theirs is a sixteenth of a value, and so is what
+  // a rounding to the other side of a border costs, which float32 does to one value in
+  // 10^5 (36864 tokens x 36 rows 102 and 108 us)
   float C[kNeed], S[kNeed];
+  double C64[EIGHT ? kNeed : 1], S64[EIGHT ? kNeed : 1];
+  if (EIGHT && has_keys) {
 #pragma unroll
-  for (int e = 0; e < kNeed; ++e) {
-    C[e] = from_lane(cs, (pair0 + e) & 63);
-    S[e] = from_lane(sn, (pair0 + e) & 63);
-    if (second) S[e] = -S[e];
+    for (int e = 0; e < (EIGHT ? kNeed : 1); ++e) {
+      C64[e] = from_lane(cs64, (pair0 + e) & 63);
+      S64[e] = from_lane(sn64, (pair0 + e) & 63);
+      if (second) S64[e] = -S64[e];
+      C[e] = (float)C64[e];
+      S[e] = (float)S64[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kNeed; ++e) {
+      C[e] = from_lane(cs, (pair0 + e) & 63);
+      S[e] = from_lane(sn, (pair0 + e) & 63);
+      if (second) S[e] = -S[e];
+    }
   }
   // pairs of this lane that turn (halves: pairs is a multiple of 8, so all or none)
   const int turning = INTERLEAVED ? p.pairs - 4 * c : (c < 2 * half_lanes ? 8 : 0);
@@ -250,6 +298,23 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(AppendParams p) {
       // as much longer where all fits the caches (append and attention of 4608
       // tokens 242.7 and 243.2 us)
       if constexpr (EIGHT) {
+        // whether some of these four rows are keys
+        if (r0 + 4 * u + 3 >= p.heads && r0 + 4 * u < p.heads + p.kv_heads) {
+          const bool is_key = turn[u] && r0 + 4 * u + sub >= p.heads;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const double a = lo_of<F16>(x[u][e]), d = hi_of<F16>(x[u][e]);
+            uint32_t w;
+            if constexpr (INTERLEAVED) {
+              w = pack<F16>((float)(a * C64[e] - d * S64[e]), (float)(a * S64[e] + d * C64[e]));
+            } else {
+              const uint32_t o = (uint32_t)__builtin_amdgcn_ds_bpermute(partner << 2, (int)x[u][e]);
+              w = pack<F16>((float)(a * C64[2 * e] - lo_of<F16>(o) * S64[2 * e]),
+                            (float)(d * C64[2 * e + 1] - hi_of<F16>(o) * S64[2 * e + 1]));
+            }
+            y[e] = is_key && (INTERLEAVED ? e < turning : turning > 0) ? w : y[e];
+          }
+        }
         uint32_t exponent;
         const u32x2 z = quantise<F16>(y, &exponent);
         if (scale_to[u]) {
