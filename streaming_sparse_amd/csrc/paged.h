@@ -1597,8 +1597,15 @@ struct Sizes {
 // longer walk of the prefix, which is then cut too little (64 x 1 token behind 16384,
 // up to 600 rows of their own: 51 us with a table of 10 pages, 69 with 32, 123 with 64,
 // 460 with 256; 16 x 1 behind 131001 128 us with 33 pages, 211 with 256).
-constexpr double kJoinStart = 3.0, kSoloPage[] = {0.85, 0.5}, kSoloLatency[] = {3.5, 2.5}, kSoloStart = 3.0,
-                 kSoloItem = 5.0;
+// Pages of 8 bits: a narrow tile's take 0.42 us, 0.92 with two workgroups on a CU, and
+// no less where a page comes from memory; a wave by itself draws one in 1.8 and a CU
+// in 0.5; an item begins and ends in 2.5 (4 x 1 token, 12 heads, behind 2000: the
+// prefix apart 12.1, joint 15.5 by the 16-bit figures); a tile over prefix and own
+// pages starts in 9.  A joint plan's lists are taken to be 0.65 full also where
+// memory bounds them (64 x 1 behind 64, up to 2000 own rows: whole lists in narrow
+// tiles 39, apart in wide ones 47).
+constexpr double kJoinStart = 3.0, kSoloPage[] = {0.85, 0.5}, kSoloLatency[] = {3.5, 1.8}, kSoloStart = 3.0,
+                 kSoloItem[] = {5.0, 2.5};
 double start_time(int T, double rows, bool singly) {
   return T == kNarrow ? 7.0 : singly ? 6.0 + 5.0 * rows / kWide : 5.0 + 3.0 * rows / kWide;
 }
@@ -1606,20 +1613,22 @@ double tile_page(int T, double rows, double active, double cus, double unshared,
                  bool two = false) {
   const double busy = active / cus;
   double page;
-  if (T == kNarrow) {
+  if (T == kNarrow && z.eight) {
+    page = 0.42 + 0.5 * std::min(1.0, std::max(0.0, busy - 1.0));
+  } else if (T == kNarrow) {
     page = 0.47 + 0.25 * std::min(1.0, std::max(0.0, busy - 1.0));
   } else {
     const double second = std::max(0.0, std::ceil(rows / 32) - 4) / 4;     // SIMDs with two waves
     const double few = two ? 1.7 : singly ? 1.3 : 1.2, more = singly ? 0.3 : 0.25;
     page = second > 0 ? few + more * std::min(1.0, busy) * second * second : two ? 1.15 : 0.95;
   }
-  return page + unshared * std::max(0.0, (z.eight ? 0.65 : T == kNarrow ? 1.2 : 1.1) - page);
+  return page + unshared * std::max(0.0, (z.eight ? 0.42 : T == kNarrow ? 1.2 : 1.1) - page);
 }
 double state_time(double rows) { return rows * 2 * (4.0 * kState / 32) / 4.5e6; }
 // Two workgroups on a CU draw less together (8 heads behind 30000 rows: 32 pieces
 // each 31.9 us, 64 38.9).
 double page_time(double pages, bool eight, double busy = 1.0) {
-  return pages * (eight ? 16512 : 32768) / 5.2e6 * (1.0 + 0.2 * std::max(0.0, busy - 1.0));
+  return pages * (eight ? 16512 / 6.0e6 : 32768 / 5.2e6) * (1.0 + 0.2 * std::max(0.0, busy - 1.0));
 }
 
 constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64, 96, 128, 192, 256};
@@ -1643,11 +1652,15 @@ int cut_in(int units, int c, int* cut) {
 // 422.  The own lists' first pieces come first, then the second ones, on the CUs the
 // prefix leaves (64 x 1 behind 2048, up to 2000 own rows: 75, list by list 85), as
 // many workgroups as there are places, each wave several items (128 x 1 behind 4096,
-// up to 1000: 80, with a workgroup for every eight items 87).
-double plan_apart(const Sizes& z, Plan* plan) {
+// up to 1000: 80, with a workgroup for every eight items 87).  In 8 bits up to 64 rows
+// may go in two narrow tiles, which both read the prefix, the second time from L2; a
+// wide tile of so few rows waits for its own barriers (16 x 1 behind 131001: 87 and
+// 113; 40 x 1, 12 heads, behind 9000: 22 and 27).  Two such tiles may share a CU (16 x 1
+// behind 20000: 24 and 28).
+double plan_apart(const Sizes& z, int T, Plan* plan) {
   const long long rows = z.rows();
-  const int T = rows <= kNarrow ? kNarrow : kWide, prefix_pages = z.prefix_pages(), table = z.own_pages(kNarrow);
-  const int slots = z.cus;
+  const int prefix_pages = z.prefix_pages(), table = z.own_pages(kNarrow);
+  const int slots = T == kNarrow && rows > T ? 2 * z.cus : z.cus;
   plan->rows = T;
   plan->row_tiles = (int)((rows + 31) / 32);
   plan->prefix_tiles = (int)((rows + T - 1) / T);
@@ -1674,7 +1687,7 @@ double plan_apart(const Sizes& z, Plan* plan) {
       const double page = std::max({kSoloLatency[z.eight], kSoloPage[z.eight] * x * (even ? 1.0 : 1.15),
                                      page_time(0.7 * groups * x, z.eight)});
       const double time =
-          kSoloStart + std::ceil(n / (groups * x)) * (kSoloItem + page * std::min<double>(cut, mean));
+          kSoloStart + std::ceil(n / (groups * x)) * (kSoloItem[z.eight] + page * std::min<double>(cut, mean));
       if (time < least) {
         least = time;
         *g = groups;
@@ -1754,7 +1767,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
   const double tiles = (double)(own_tiles - whole);
   const double full = std::min<double>(per_seq, T);         // rows of the fullest tile
   const double live = per_seq / std::ceil(per_seq / T);     // and of the mean one
-  const double start = start_time(T, live, singly);
+  const double start = start_time(T, live, singly) + (z.eight && !wide ? 2.0 : 0.0);
   // the part of all lists' pages that come from memory, and of a list that no other
   // tile reads
   const double read = std::min(1.0, z.kv_heads * (z.prefix_pages() + (double)z.batch * table) /
@@ -1779,7 +1792,7 @@ double plan_joint(const Sizes& z, int T, Plan* plan) {
       const double active = std::min(tiles * pieces, (double)slots);
       time = std::ceil(tiles * pieces / slots) *
              (start + std::max(cut * tile_page(T, full, active, z.cus, unshared, singly, z),
-                               page_time(read * active * cut, z.eight, active / z.cus)));
+                               page_time(read * active * cut * (z.eight ? 0.65 : 1.0), z.eight, active / z.cus)));
       states = pieces > 1 ? tiles * pieces : 0.0;
     }
     const double cost = time + (states > 0 ? state_time(states * live) + kJoinStart : 0.0);
@@ -1810,7 +1823,11 @@ int make_plan(Sizes z, Plan* plan) {
       }
     };
     if (!z.few()) consider(plan_joint(z, kHalfWide, &other));
-    if (z.batch > 1 && z.prefix_tokens > 0) consider(plan_apart(z, &other));
+    if (z.batch > 1 && z.prefix_tokens > 0) {
+      const bool narrow = z.rows() <= kNarrow;
+      consider(plan_apart(z, narrow ? kNarrow : kWide, &other));
+      if (z.eight && !narrow && z.rows() <= 2 * kNarrow) consider(plan_apart(z, kNarrow, &other));
+    }
     last_plan = joint;
     last_sizes = z;
   }
