@@ -1011,15 +1011,27 @@ template <bool PAIRS>
 constexpr int kRing = PAIRS ? 5 : 4;
 
 // What a lane has taken of an 8-bit page on its way to LDS: 16 values of K and of V,
-// their rows' exponents.
+// their rows' exponents, and that of V's row `lane`.
 struct Staged {
   u32x4 k, v;
-  uint32_t ks, vs;
+  uint32_t ks, vs, all;
 };
+
+// V's 8-bit values against bf16 queries where two parts are asked for (RELATIVE).  Two
+// bf16 parts of a probability are half as many products again as one; one fp16 part has
+// 11 bits, beside which an output's 8 are all that counts (against 64 bits both 0.00166),
+// and 8-bit values are exact in fp16, but not their powers of two.  So V goes to LDS in
+// units of 2^E, one E for all pages so far (when it rises the sums follow), in which
+// values of the exponents E - 15 .. E are exact.  From the first page on that has other
+// ones, seen or not, pages go as bf16 in units of 1 and meet two bf16 parts, in a loop of
+// its own (as a branch in the first one it took its registers: 64 x 1 token behind 16384
+// 127 us).  64 x 1 behind 16384: 42.1 us, by two bf16 parts 46.7.
+constexpr int kUnitLow = 127 - 40, kUnitHigh = 127 + 40, kUnitSpan = 15;      // as floats' exponents
 
 template <class How, bool PAIRS, bool TWO>
 __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
-  constexpr bool F16 = How::F16, Q8 = How::Q8, SHAPED = How::SHAPED;
+  constexpr bool F16 = How::F16, Q8 = How::Q8, SHAPED = How::SHAPED, RELATIVE = Q8 && !F16 && TWO,
+                 V16 = F16 || RELATIVE;
   constexpr int kSlots = kRing<PAIRS>;
   const int r = lane & 31, hh = lane >> 5;
   Sight x;
@@ -1076,6 +1088,10 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   // in them: a lane takes 16 dims of row 8 wave + lane / 8.
   Staged staged[2];
   const uint8_t* const sh = Q8 ? p.scales + (long long)j.h * p.s_head + 8 * wave + (lane >> 3) : nullptr;
+  const uint8_t* const every = RELATIVE ? p.scales + (long long)j.h * p.s_head + kPage + lane : nullptr;
+  int unit = kUnitLow;                  // E of the pages in LDS, as a float's exponent
+  int units[3] = {kUnitLow, kUnitLow, kUnitLow};       // of units u .. u + 2
+  int fine_end = end;                   // units that are landed as fp16
   auto fetch = [&](int u, Staged& to) {
     if (u >= end) return 0;
     const Unit x = list.at(p, j, u, lane);
@@ -1085,18 +1101,36 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     to.v = *reinterpret_cast<const u32x4*>(vh + page * p.kv_tok + at);
     to.ks = sh[page * p.s_page];
     to.vs = sh[page * p.s_page + kPage];
+    if constexpr (RELATIVE) to.all = every[page * p.s_page];
     return x.rows;
   };
   auto land = [&](int u, int slot, const Staged& from, int rows) {
-    if (u >= end) return;
-    const int row = 8 * wave + (lane >> 3), c = 2 * (lane & 7);
+    if (u >= end) return unit;
+    const int row = 8 * wave + (lane >> 3), c = 2 * (lane & 7), low = low_of(u);
+    if constexpr (RELATIVE) {
+      // the same in every wave
+      const bool seen = lane < rows && lane >= low;
+      const int e = (int)from.all;
+      if (u < fine_end) {
+        for (uint64_t more; unit < kUnitHigh && (more = __ballot(seen && e > unit));)
+          unit = min(__builtin_amdgcn_readlane(e, __builtin_ctzll(more)), kUnitHigh);
+        if (__ballot(seen && (e > unit || e < unit - kUnitSpan))) fine_end = u;
+      }
+      if (u >= fine_end) unit = 127;
+    }
     lds_u8* const kt = kring + slot * kTile + row * 256;
     lds_u8* const vt = vring + slot * kTile + row * 256;
-    const float ks = __uint_as_float(from.ks << 23), vs = __uint_as_float(from.vs << 23);
+    const float ks = __uint_as_float(from.ks << 23), vs = __uint_as_float((RELATIVE ? from.vs + 127 - unit : from.vs) << 23);
     *(lds_u32x4*)(kt + ((c ^ (row & 15)) << 4)) = widen<F16>(from.k[0], from.k[1], ks);
     *(lds_u32x4*)(kt + (((c + 1) ^ (row & 15)) << 4)) = widen<F16>(from.k[2], from.k[3], ks);
-    u32x4 a = widen<F16>(from.v[0], from.v[1], vs), b = widen<F16>(from.v[2], from.v[3], vs);
-    const int low = low_of(u);
+    u32x4 a, b;
+    if (RELATIVE && u >= fine_end) {
+      a = widen<false>(from.v[0], from.v[1], vs);
+      b = widen<false>(from.v[2], from.v[3], vs);
+    } else {
+      a = widen<V16>(from.v[0], from.v[1], vs);
+      b = widen<V16>(from.v[2], from.v[3], vs);
+    }
     if (rows < kPage || low > 0) {
       // as clear_rows
       const bool there = row < rows && row >= low;
@@ -1105,6 +1139,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     }
     *(lds_u32x4*)(vt + ((c ^ vswz(row)) << 4)) = a;
     *(lds_u32x4*)(vt + (((c + 1) ^ vswz(row)) << 4)) = b;
+    return unit;
   };
   auto issue = [&](int u) {
     if (u >= end) return 0;
@@ -1123,8 +1158,8 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
 #pragma unroll
     for (int i = 0; i < 2; ++i) rows_ahead[2 + i] = fetch(begin + 2 + i, staged[i]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) land(begin + i, i, first[i], rows_ahead[i]);
-    loads_left<0>();            // the query rows too
+    for (int i = 0; i < 2; ++i) units[i] = land(begin + i, i, first[i], rows_ahead[i]);
+    if (begin >= end) loads_left<0>();          // the query rows came before the first page's
   } else {
     rows_ahead[0] = issue(begin);
     rows_ahead[1] = issue(begin + 1);
@@ -1144,7 +1179,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
   // the running maximum in log2 units; the exponents' offset and the raw score
   // that the accumulators are rescaled beyond, which change with it alone
-  float m = -INFINITY, nb = kLift<F16>, beyond = -INFINITY, ls = 0.0f, mx;
+  float m = -INFINITY, nb = kLift<V16>, beyond = -INFINITY, ls = 0.0f, mx;
   const float slack = kSlack / per_score;
   const uint32_t klane = (uint32_t)(r * 256 + ((hh ^ (r & 15)) << 4));
   uint32_t vlane;
@@ -1191,7 +1226,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
       m = to;
-      nb = kLift<F16> - at;
+      nb = kLift<V16> - at;
       beyond = __builtin_fmaxf(beyond - slack, mx) + slack;
     }
   };
@@ -1204,10 +1239,12 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
   auto kread = [&](int slot, int half, int x) {
     return *(lds_u32x4*)(kat[x] + slot * kTile + half * (kTile / 2));
   };
-  auto half_step = [&](auto slot_c, auto half_c, const f32x16& Sc, f32x16& Sn, int next, int next_rows) {
-    constexpr int slot = decltype(slot_c)::value, half = decltype(half_c)::value;
-    constexpr int nslot = (slot + half) % kSlots, nhalf = half ^ 1;            // the next half page
-    constexpr int aslot = (slot + 1) % kSlots, ahalf = half;                   // and the one after
+  auto half_step = [&](auto slot, auto half_c, auto coarse_c, const f32x16& Sc, f32x16& Sn, int next, int next_rows) {
+    constexpr int half = decltype(half_c)::value;
+    constexpr bool coarse = decltype(coarse_c)::value, two = TWO && !RELATIVE || coarse, V = V16 && !coarse;
+    constexpr int nhalf = half ^ 1, ahalf = half;
+    const int nslot = (slot + half) % kSlots;            // the next half page
+    const int aslot = (slot + 1) % kSlots;                   // and the one after
     u32x4 va[2][4], pb[2], pl[2];       // pl: the second parts
     float P[16];
     auto vread = [&](int ks, int dt) {
@@ -1218,12 +1255,12 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
       P[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(Sc[i], per_score, nb));
       ls += P[i];
       if (!(i & 1)) return;
-      if constexpr (TWO) {
-        const u32x2 x = split2<F16>(P[i - 1], P[i]);
+      if constexpr (two) {
+        const u32x2 x = split2<V>(P[i - 1], P[i]);
         pb[i >> 3][(i & 7) >> 1] = x[0];
         pl[i >> 3][(i & 7) >> 1] = x[1];
       } else {
-        pb[i >> 3][(i & 7) >> 1] = pack2<F16>(P[i - 1], P[i]);
+        pb[i >> 3][(i & 7) >> 1] = pack2<V>(P[i - 1], P[i]);
       }
     };
     Sn = f32x16{};
@@ -1240,8 +1277,8 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
-      O[dt] = mma<F16>(va[0][dt], pb[0], O[dt]);
-      if constexpr (TWO) O[dt] = mma<F16>(va[0][dt], pl[0], O[dt]);
+      O[dt] = mma<V>(va[0][dt], pb[0], O[dt]);
+      if constexpr (two) O[dt] = mma<V>(va[0][dt], pl[0], O[dt]);
       va[1][dt] = vread(1, dt);
       expo(8 + 2 * dt);
       expo(9 + 2 * dt);
@@ -1249,14 +1286,15 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     asm volatile("" : "+v"(ls));   // the sums here, not behind the branches below
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
-      O[dt] = mma<F16>(va[1][dt], pb[1], O[dt]);
-      if constexpr (TWO) O[dt] = mma<F16>(va[1][dt], pl[1], O[dt]);
+      O[dt] = mma<V>(va[1][dt], pb[1], O[dt]);
+      if constexpr (two) O[dt] = mma<V>(va[1][dt], pl[1], O[dt]);
       ka[dt] = kread(aslot, ahalf, dt);
     }
     settle(Sn, next, nhalf, next_rows);
     rescale();
   };
 
+  int held = kUnitLow;       // E of the sums
   if (begin < end) {
     // The first steps' pages: K and V of one (two), and K of the next; each unit is 2
     // loads of K, then 2 of V.
@@ -1280,25 +1318,36 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
 #pragma unroll
     for (int st = 0; st < 4; ++st) ka[st] = kread(0, 1, st);
     int u = begin;
-    auto step = [&](auto slot_c) {
+    held = units[0];
+    auto step = [&](auto slot, auto coarse) {
       constexpr std::integral_constant<int, 0> low;
       constexpr std::integral_constant<int, 1> high;
       f32x16 S1;
-      if (alive) half_step(slot_c, low, S, S1, u, rows_ahead[0]);
+      if constexpr (RELATIVE) {
+        if (units[0] != held) {
+          const float a = __uint_as_float((uint32_t)(127 + held - units[0]) << 23);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
+          held = units[0];
+        }
+      }
+      if (alive) half_step(slot, low, coarse, S, S1, u, rows_ahead[0]);
       if constexpr (Q8) {
-        constexpr int slot = decltype(slot_c)::value;
-        land(u + 2, (slot + 2) % kSlots, staged[slot & 1], rows_ahead[2]);
-        rows_ahead[4] = fetch(u + 4, staged[slot & 1]);
+        // the coarse loop's slots are not known here: its next page is staged[0] always
+        const int i = coarse ? 0 : slot & 1;
+        units[2] = land(u + 2, (slot + 2) % kSlots, staged[i], rows_ahead[2]);
+        if constexpr (coarse) staged[0] = staged[1];
+        rows_ahead[4] = fetch(u + 4, staged[coarse ? 1 : i]);
       } else {
         rows_ahead[3] = issue(u + 3);
       }
-      if (alive) half_step(slot_c, high, S1, S, u + 1, rows_ahead[1]);
+      if (alive) half_step(slot, high, coarse, S1, S, u + 1, rows_ahead[1]);
       if constexpr (PAIRS) {
-        constexpr std::integral_constant<int, (decltype(slot_c)::value + 1) % kSlots> slot_d;
+        constexpr std::integral_constant<int, (slot + 1) % kSlots> slot_d;
         rows_ahead[4] = issue(u + 4);
         if (alive && u + 1 < end) {
-          half_step(slot_d, low, S, S1, u + 1, rows_ahead[1]);
-          half_step(slot_d, high, S1, S, u + 2, rows_ahead[2]);
+          half_step(slot_d, low, coarse, S, S1, u + 1, rows_ahead[1]);
+          half_step(slot_d, high, coarse, S1, S, u + 2, rows_ahead[2]);
         }
       }
       if constexpr (!Q8) {
@@ -1310,26 +1359,42 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
       u += kStep;
 #pragma unroll
       for (int i = 0; i < (Q8 ? 4 : 3); ++i) rows_ahead[i] = rows_ahead[i + kStep];
+      units[0] = units[1];
+      units[1] = units[2];
       if constexpr (!Q8) {
         if (u < end) clear_rows(u, rows_ahead[0]);
         if (PAIRS && u + 1 < end) clear_rows(u + 1, rows_ahead[1]);
       }
       meet();
-      return u < end;
+      return u < (coarse || !RELATIVE ? end : fine_end);
     };
     auto slot = [](auto k) { return std::integral_constant<int, decltype(k)::value * kStep % kSlots>{}; };
-    bool more = true;
+    constexpr std::false_type fine;
+    bool more = !RELATIVE || begin < fine_end;
     while (more) {
-      more = step(slot(std::integral_constant<int, 0>{})) && step(slot(std::integral_constant<int, 1>{})) &&
-             step(slot(std::integral_constant<int, 2>{})) && step(slot(std::integral_constant<int, 3>{}));
-      if constexpr (PAIRS) more = more && step(slot(std::integral_constant<int, 4>{}));
+      more = step(slot(std::integral_constant<int, 0>{}), fine) && step(slot(std::integral_constant<int, 1>{}), fine) &&
+             step(slot(std::integral_constant<int, 2>{}), fine) && step(slot(std::integral_constant<int, 3>{}), fine);
+      if constexpr (PAIRS) more = more && step(slot(std::integral_constant<int, 4>{}), fine);
+    }
+    if constexpr (RELATIVE) {
+      if (u < end && (u - begin) & 1) {
+        const Staged x = staged[0];
+        staged[0] = staged[1];
+        staged[1] = x;
+      }
+      while (u < end) step((u - begin) % kSlots, std::true_type{});
     }
   }
 
   // the lane's row, formed anew so that no register holds it across the loop
   int e = lane;
   asm volatile("" : "+v"(e));
-  const float M = m == -INFINITY ? m : m - kLift<F16>, l = half_sum(ls);
+  const float M = m == -INFINITY ? m : m - kLift<V16>, l = half_sum(ls);
+  if constexpr (RELATIVE) {
+    const float a = __uint_as_float((uint32_t)held << 23);
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
+  }
   if (j.state >= 0) {
     write_state(p, j, O, M, l, wave, e);
     return;

@@ -349,6 +349,61 @@ def test_attention_large(device, batch, new, held, heads, kv_heads, prefix, caus
         c.check(*c.attend(causal, single_av=parts), causal, score=2.0 ** -13 + 2.0 ** -10)
 
 
+@pytest.mark.parametrize('new,held,heads,kv_heads,prefix', [
+    pytest.param([1] * 70, 100, 8, 2, 2500, id='apart'),
+    pytest.param([150, 90], 70, 3, 1, 321, id='joint'),
+])
+@pytest.mark.parametrize('powers', ['alike', 'rising', 'falling', 'one_page', 'one_row', 'first_page', 'wide_apart', 'tiny',
+                                    'huge', 'zeros', 'edges'])
+def test_attention_powers_of_two_of_values(device, new, held, heads, kv_heads, prefix, powers):
+    """Two-part wide tiles hold the values relative to the largest power of two so far
+    where that is exact: rows within and outside that range, in any order."""
+    c = Case(device, new, [held] * len(new), heads, kv_heads, prefix)
+    s = c.cache.scales[:, :, 1]
+    live = s != 255
+    order = c.prefix.tolist()
+    at = torch.zeros(s.shape[0], dtype=torch.long, device=device)           # a page's place in its list
+    for i, p in enumerate(order):
+        at[p] = i
+    for row in c.table.tolist():
+        for i, p in enumerate(row):
+            if p >= 0:
+                at[p] = len(order) + i
+    place = 64 * at[:, None] + torch.arange(64, device=device)              # [P, 64]
+    e = torch.full_like(place, 124)
+    if powers == 'rising':
+        e = 60 + place // 24
+    elif powers == 'falling':
+        e = 200 - place // 24
+    elif powers == 'one_page':
+        e = torch.where(at[:, None] == 3, 100 + torch.arange(64, device=device), e)
+    elif powers == 'one_row':                   # one that no query gives weight
+        e = torch.where(place == 200, 240, e)
+    elif powers == 'first_page':
+        e = torch.where(at[:, None] == 0, torch.arange(64, device=device) * 3 + 40, e)
+    elif powers == 'wide_apart':
+        e = torch.where(place % 2 == 0, 30, 230)
+    elif powers == 'tiny':
+        e = torch.full_like(place, 3) + place % 9
+    elif powers == 'huge':
+        e = torch.full_like(place, 225) + place % 9
+    elif powers == 'edges':                     # just inside the range of one power and just outside it
+        e = torch.where(at[:, None] < 3, 124 - place % 16, 124 - place % 17)
+    s.copy_(torch.where(live, e.to(torch.uint8)[:, None].expand_as(s), s))
+    if powers == 'zeros':
+        zero = live & (place % 5 == 0)[:, None]
+        c.cache.v.view(torch.uint8).masked_fill_(zero[..., None], 0)
+        s.masked_fill_(zero, 1)
+    if powers == 'one_row':
+        page = order[200 // 64]
+        # every query's score with it is about -317, others' within 16 of 0
+        c.q[:] = 4.0 * (0.25 + 0.01 * c.q)
+        c.cache.k[page, :, 200 % 64] = -448.0
+        c.cache.scales[page, :, 0, 200 % 64] = 123
+    for single in (False, None):
+        c.check(*c.attend(single_av=single), score=2.0 ** -13 + 2.0 ** -10)
+
+
 def test_attention_powers_of_two_far_apart(device):
     """Values from 2^-80 to 2^80 in rows next to each other, keys whose powers
     nearly cancel the queries': the largest rule, nothing is lost or infinite."""
