@@ -670,14 +670,28 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
   asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
 
+// V's 8-bit values against bf16 queries where a probability has two parts (RELATIVE).  Two
+// bf16 parts are half as many products again as one; one fp16 part has 11 bits, beside
+// which an output's 8 are all that counts (against 64 bits both 0.00166), and 8-bit
+// values are exact in fp16, but not their powers of two.  So V counts in units of 2^E,
+// one E for all pages so far (when it rises the sums follow), in which values of the
+// exponents E - 15 .. E are exact in fp16.  From the first page on that has other ones,
+// pages meet two bf16 parts in units of 1, in a loop of its own (as a branch in a wide
+// tile's first one it took its registers: 64 x 1 token behind 16384 127 us).  64 x 1
+// behind 16384 42.2 us, by two bf16 parts 46.7; 16 x 1 behind 131001 76 and 85; 64 x 1
+// behind 64, up to 2000 own rows, 33 and 36.5.  Waves by themselves, which wait for
+// their pages, keep the two parts: a second loop beside the prefix tiles' costs more
+// than it saves (4 x 1, 12 heads, behind 2000 12.7 and 11.9).
+constexpr int kUnitLow = 127 - 40, kUnitHigh = 127 + 40, kUnitSpan = 15;      // as floats' exponents
+
 // A wave's walk over a tile's 8-bit pages: pages w, w + NW, ... of the list, 8 KB of K
 // and as much of V at a time.  16-byte chunk c of row r lies at c ^ swz8(r), with which
 // neither the rows that 16 lanes read nor the transposing reads meet on a bank.
 //
 // K's powers of two go into its values on their way to 16 bits.  V's operand holds
 // eight rows of one dim, so the powers go into the probabilities, p v = (p 2^e)
-// (v / 2^e), which meet V in bf16 whatever the queries' type: its range holds every
-// power of two and two parts carry more bits than an fp16 output.  Score S[i] is key 16
+// (v / 2^e), which, but for RELATIVE pages, meet V in bf16 whatever the queries' type:
+// its range holds every power of two and two parts carry more bits than an fp16 output.  Score S[i] is key 16
 // (i / 8) + 8 hh + i % 8 of its half page (the K operand's rows are taken in that
 // order), so that a lane's probabilities belong to the eight rows of an operand.
 constexpr int kWave8 = 2 * kPage * kHeadDim + 512;     // K, V, the exponents as they come, V's as floats
@@ -686,7 +700,7 @@ __device__ __forceinline__ int swz8(int row) { return (row & 6) | ((row >> 3) & 
 template <class How, int NW>
 __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave,
                                       f32x16 (&O)[4], float& m, float& ls) {
-  constexpr bool F16 = How::F16, SHAPED = How::SHAPED;
+  constexpr bool F16 = How::F16, SHAPED = How::SHAPED, RELATIVE = !F16 && NW > 1;
   typedef __attribute__((address_space(3))) float lds_f32;
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
   const int r = lane & 31, hh = lane >> 5;
@@ -741,14 +755,15 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
     issue_keys(u);
     issue(vh, u, vb);
   }
-  for (; pu < j.end; pu += NW) {
+  int unit = 0;               // E of the sums, once there are any
+  // Page pu; with `fine` false, nothing done, where its powers of two are too far apart.
+  auto step = [&](auto fine_c) {
+    constexpr bool fine = RELATIVE && decltype(fine_c)::value;
     const bool more = pu + NW < j.end;
     const bool own = pu >= j.prefix_pages;
     const int at = kPage * (pu - (own ? j.prefix_pages - j.skip : 0));       // its first row in the prefix, or of its own
     const int low = SHAPED && own ? j.low - at : 0;
     loads_left<8>();                                        // K and the exponents landed, V behind them
-    // rows behind the end, or before every window, hold anything, their exponents too
-    vscale[lane] = lane < u.rows && lane >= low ? exponent(raw[kPage + lane]) : 0.0f;
     f32x16 S[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -760,6 +775,27 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
         S[h] = mma<F16>(widen<F16>(w[0], w[1], scale), qop[2 * t], S[h]);
         S[h] = mma<F16>(widen<F16>(w[2], w[3], scale), qop[2 * t + 1], S[h]);
       }
+    }
+    // (while the products run) rows behind the end, or before every window, hold
+    // anything, their exponents too
+    const bool seen = lane < u.rows && lane >= low;
+    if constexpr (RELATIVE) {
+      const int e = raw[kPage + lane];
+      int to = fine ? max(unit, kUnitLow) : 127;
+      if constexpr (fine) {
+        for (uint64_t up; to < kUnitHigh && (up = __ballot(seen && e > to));)
+          to = min(__builtin_amdgcn_readlane(e, __builtin_ctzll(up)), kUnitHigh);
+        if (__builtin_expect(__ballot(seen && (e > to || e < to - kUnitSpan)) != 0, 0)) return false;
+      }
+      if (to != unit && unit > 0) {
+        const float a = __uint_as_float((uint32_t)(127 + unit - to) << 23);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
+      }
+      unit = to;
+      vscale[lane] = seen ? exponent(e + 127 - to) : 0.0f;
+    } else {
+      vscale[lane] = seen ? exponent(raw[kPage + lane]) : 0.0f;
     }
     Unit after{-1, 0};
     if (more) {
@@ -787,7 +823,7 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
       for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
       m = to;
     }
-    const float nb = m == -INFINITY ? 0.0f : -m;
+    const float nb = kLift<RELATIVE> - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -815,20 +851,25 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
         const f32x4 f = *(lds_f32x4*)(vscale + 16 * ks + 8 * hh + 4 * half);
         const f32x16& P = S[ks >> 1];
         const int i = 8 * (ks & 1) + 4 * half;
-        const u32x2 a = split2<false>(P[i] * f[0], P[i + 1] * f[1]), b = split2<false>(P[i + 2] * f[2], P[i + 3] * f[3]);
-        hi[2 * half] = a[0];
-        hi[2 * half + 1] = b[0];
-        lo[2 * half] = a[1];
-        lo[2 * half + 1] = b[1];
+        if constexpr (fine) {
+          hi[2 * half] = pack2<true>(P[i] * f[0], P[i + 1] * f[1]);
+          hi[2 * half + 1] = pack2<true>(P[i + 2] * f[2], P[i + 3] * f[3]);
+        } else {
+          const u32x2 a = split2<false>(P[i] * f[0], P[i + 1] * f[1]), b = split2<false>(P[i + 2] * f[2], P[i + 3] * f[3]);
+          hi[2 * half] = a[0];
+          hi[2 * half + 1] = b[0];
+          lo[2 * half] = a[1];
+          lo[2 * half + 1] = b[1];
+        }
       }
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) {
         // dim 32 dt + lane % 32 of the same keys
         const int g = lane >> 4, i = lane & 15, row = 16 * ks + 8 * (g >> 1) + (i >> 1);
         const u32x2 w = tr8(vb + row * 128 + (((2 * dt + (g & 1)) ^ swz8(row)) << 4) + (i & 1) * 8);
-        const u32x4 va = widen<false>(w[0], w[1], 1.0f);
-        O[dt] = mma<false>(va, hi, O[dt]);
-        O[dt] = mma<false>(va, lo, O[dt]);
+        const u32x4 va = widen<fine>(w[0], w[1], 1.0f);
+        O[dt] = mma<fine>(va, hi, O[dt]);
+        if constexpr (!fine) O[dt] = mma<false>(va, lo, O[dt]);
       }
     }
     if (more) {
@@ -836,6 +877,18 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
       issue(vh, after, vb);
     }
     u = after;
+    pu += NW;
+    return true;
+  };
+  if constexpr (RELATIVE) {
+    while (pu < j.end && step(std::true_type{})) {
+    }
+  }
+  while (RELATIVE ? __builtin_expect(pu < j.end, 0) : pu < j.end) step(std::false_type{});
+  if constexpr (RELATIVE) {
+    const float a = __uint_as_float((uint32_t)unit << 23);
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
   }
 }
 
@@ -846,7 +899,7 @@ constexpr int kWaveBytes = How::Q8 ? kWave8 : 2 * kHalf;      // a narrow wave's
 template <class How, int NW>
 __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
   constexpr bool F16 = How::F16;
-  constexpr float lift = How::Q8 ? 0.0f : kLift<F16>;
+  constexpr float lift = kLift<How::Q8 ? !F16 && NW != 1 : F16>;
   f32x16 O[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
@@ -1016,17 +1069,6 @@ struct Staged {
   u32x4 k, v;
   uint32_t ks, vs, all;
 };
-
-// V's 8-bit values against bf16 queries where two parts are asked for (RELATIVE).  Two
-// bf16 parts of a probability are half as many products again as one; one fp16 part has
-// 11 bits, beside which an output's 8 are all that counts (against 64 bits both 0.00166),
-// and 8-bit values are exact in fp16, but not their powers of two.  So V goes to LDS in
-// units of 2^E, one E for all pages so far (when it rises the sums follow), in which
-// values of the exponents E - 15 .. E are exact.  From the first page on that has other
-// ones, seen or not, pages go as bf16 in units of 1 and meet two bf16 parts, in a loop of
-// its own (as a branch in the first one it took its registers: 64 x 1 token behind 16384
-// 127 us).  64 x 1 behind 16384: 42.1 us, by two bf16 parts 46.7.
-constexpr int kUnitLow = 127 - 40, kUnitHigh = 127 + 40, kUnitSpan = 15;      // as floats' exponents
 
 template <class How, bool PAIRS, bool TWO>
 __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {

@@ -352,11 +352,14 @@ def test_attention_large(device, batch, new, held, heads, kv_heads, prefix, caus
 @pytest.mark.parametrize('new,held,heads,kv_heads,prefix', [
     pytest.param([1] * 70, 100, 8, 2, 2500, id='apart'),
     pytest.param([150, 90], 70, 3, 1, 321, id='joint'),
+    pytest.param([1] * 6, 300, 4, 2, 2500, id='narrow_apart'),
+    pytest.param([1], 3000, 4, 2, 0, id='narrow'),
+    pytest.param([2] * 3, 500, 8, 2, 321, id='narrow_joint'),
 ])
 @pytest.mark.parametrize('powers', ['alike', 'rising', 'falling', 'one_page', 'one_row', 'first_page', 'wide_apart', 'tiny',
                                     'huge', 'zeros', 'edges'])
 def test_attention_powers_of_two_of_values(device, new, held, heads, kv_heads, prefix, powers):
-    """Two-part wide tiles hold the values relative to the largest power of two so far
+    """Tiles with two parts hold the values relative to the largest power of two so far
     where that is exact: rows within and outside that range, in any order."""
     c = Case(device, new, [held] * len(new), heads, kv_heads, prefix)
     s = c.cache.scales[:, :, 1]
@@ -395,7 +398,7 @@ def test_attention_powers_of_two_of_values(device, new, held, heads, kv_heads, p
         c.cache.v.view(torch.uint8).masked_fill_(zero[..., None], 0)
         s.masked_fill_(zero, 1)
     if powers == 'one_row':
-        page = order[200 // 64]
+        page = (order + c.table[0].tolist())[200 // 64]
         # every query's score with it is about -317, others' within 16 of 0
         c.q[:] = 4.0 * (0.25 + 0.01 * c.q)
         c.cache.k[page, :, 200 % 64] = -448.0
