@@ -48,7 +48,9 @@ int ssa_paged8_read(const void* cache_k, const void* cache_v, long long kv_page_
                     hipStream_t stream);
 
 /* ssa_paged_attention over an 8-bit cache.  In tiles of up to 32 rows a probability
- * meets V in two bf16 parts whatever the queries' type. */
+ * meets V in two parts, whatever the flags.  Where there are two and the queries are
+ * bf16 they may be one of fp16 instead, which carries 11 bits (values whose powers of
+ * two lie within 2^15 of the largest of the pages walked before). */
 int ssa_paged8_attention(const void* q, long long q_token_stride, long long q_head_stride, const void* cache_k,
                          const void* cache_v, long long kv_page_stride, long long kv_head_stride, const void* scales,
                          long long scales_page_stride, long long scales_head_stride, const int32_t* prefix,
@@ -66,7 +68,8 @@ int ssa_paged8_attention(const void* q, long long q_token_stride, long long q_he
  *   window > 0:   of its own sequence a query sees the rows j > lengths[b] - n + i -
  *                 window only.  Pages that no query sees may be absent, their rows
  *                 anything.
- * 0 <= cap < infinity, 0 <= window < 2^30. */
+ * 0 <= cap <= 65536, 0 <= window < 2^30; slopes are finite.  A score is off by up to 2^-22
+ * of the cap. */
 int ssa_paged_attention_shaped(const void* q, long long q_token_stride, long long q_head_stride, const void* cache_k,
                                const void* cache_v, long long kv_token_stride, long long kv_head_stride,
                                const int32_t* prefix, int prefix_tokens, const int32_t* table, const int32_t* lengths,

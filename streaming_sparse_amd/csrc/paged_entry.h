@@ -4,9 +4,10 @@
 
 namespace {
 
-// cap 0: none; slopes null: none; window 0: none.
-bool shape_fits(float cap, const float* slopes, int window) {
-  return cap >= 0.0f && cap < INFINITY && window >= 0 && window < (1 << 30) && !((uintptr_t)slopes & 3);
+// cap 0: none; slopes null: none; window 0: none.  A score's error is 2^-22 of the cap,
+// 2^-6 at the largest that is taken.
+bool shape_fits(float scale, float cap, const float* slopes, int window) {
+  return cap >= 0.0f && cap <= 65536.0f && (cap == 0.0f || 2.0f * kLog2e * scale / cap < INFINITY) && window >= 0 && window < (1 << 30) && !((uintptr_t)slopes & 3);
 }
 
 void set_shape(PagedParams* p, float scale, float cap, const float* slopes, int window) {
@@ -42,7 +43,7 @@ int attend16(const void* q, long long q_token_stride, long long q_head_stride, c
   p.pages = pages;
   const Sizes z{0, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr, (flags & 2) != 0};
   // 16-byte row pieces; a page's byte offsets fit 32 bits
-  if (!call_fits(p, z, scale, flags) || !shape_fits(cap, slopes, window) || ((kv_token_stride | kv_head_stride) & 7) ||
+  if (!call_fits(p, z, scale, flags) || !shape_fits(scale, cap, slopes, window) || ((kv_token_stride | kv_head_stride) & 7) ||
       (kv_token_stride | kv_head_stride) < 0 || kv_token_stride < kHeadDim || kv_token_stride >= (1ll << 24))
     return (int)hipErrorInvalidValue;
   set_shape(&p, scale, cap, slopes, window);
@@ -79,7 +80,7 @@ int attend8(const void* q, long long q_token_stride, long long q_head_stride, co
   p.pages = pages;
   const Sizes z{0, tokens, batch, heads, kv_heads, prefix_tokens, table_pages, starts != nullptr, (flags & 2) != 0};
   // 16-byte pieces of rows, 4-byte pieces of exponents
-  if (!call_fits(p, z, scale, flags) || !shape_fits(cap, slopes, window) || !scales || ((uintptr_t)scales & 3) ||
+  if (!call_fits(p, z, scale, flags) || !shape_fits(scale, cap, slopes, window) || !scales || ((uintptr_t)scales & 3) ||
       ((scales_page_stride | scales_head_stride) & 3) || (scales_page_stride | scales_head_stride) < 0 ||
       ((kv_page_stride | kv_head_stride) & 15) || (kv_page_stride | kv_head_stride) < 0)
     return (int)hipErrorInvalidValue;

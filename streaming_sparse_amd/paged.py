@@ -257,8 +257,8 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     and fp16 values within 2^-11 of the type's largest, may come out infinite.
 
     Shaped scores, each for itself or together, of s = scale q.k:
-    cap (positive): s becomes cap tanh(s / cap), within 2^-22 of the cap;
-    slopes [H] float32: s falls by the head's slope times the distance in rows
+    cap (up to 65536): s becomes cap tanh(s / cap), within 2^-22 of the cap;
+    slopes [H] float32, finite: s falls by the head's slope times the distance in rows
     between query and key, query i's own row being lengths[b] - n + i and the
     prefix's rows lying before row 0 (keys behind the query count alike);
     window (1 or more): of its own sequence a query sees only the `window` rows up
@@ -278,8 +278,8 @@ def _shape(cap, slopes, window, heads, dev):
     """The entries' cap, slopes and window."""
     if cap is None:
         cap = 0.0
-    elif not 0.0 < cap < math.inf:
-        raise ValueError("cap must be positive")
+    elif not 2.0 ** -126 <= cap <= 65536.0:
+        raise ValueError("cap must be positive, 65536 at most")
     slopes_ptr = None
     if slopes is not None:
         if slopes.dtype is not torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous() or \
@@ -288,7 +288,7 @@ def _shape(cap, slopes, window, heads, dev):
         slopes_ptr = slopes.data_ptr()
     if window is None:
         window = 0
-    elif window < 1 or window != int(window):
+    elif not 1 <= window < math.inf or window != int(window):
         raise ValueError("window must be a whole number from 1 on")
     return cap, slopes_ptr, min(int(window), _MOST_ROWS)
 

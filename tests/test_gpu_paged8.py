@@ -323,6 +323,8 @@ def test_attention(device, new, before, heads, kv_heads, prefix, causal, dtype):
 @pytest.mark.parametrize('batch,new,held,heads,kv_heads,prefix,causal,dtype', [
     # every way through the kernels
     pytest.param(8, 1, 200, 8, 8, 9000, True, BF16, id='apart_narrow'),
+    pytest.param(11, 1, 200, 12, 4, 9000, True, BF16, id='apart_two_narrow_33'),
+    pytest.param(21, 1, 700, 6, 2, 20000, False, FP16, id='apart_two_narrow_63'),
     pytest.param(9, 1, 200, 3, 1, 5000, True, FP16, id='joint_narrow_pieces'),
     pytest.param(1, 1, 30, 8, 2, 30000, True, BF16, id='joint_narrow_many_pieces'),
     pytest.param(40, 3, 400, 12, 12, 0, True, FP16, id='joint_narrow_whole'),

@@ -75,6 +75,7 @@ LARGE = [
     pytest.param(9, 1, 5000, 3, 1, 500, True, FP16, dict(window=1000), id='narrow_pieces'),
     pytest.param(1, 1, 30000, 8, 2, 70, True, BF16, dict(cap=50.0, window=20000), id='narrow_many_pieces'),
     pytest.param(40, 3, 400, 12, 12, 0, True, FP16, dict(slopes=True, window=100), id='narrow_whole'),
+    pytest.param(12, 1, 700, 8, 2, 9000, True, BF16, dict(cap=50.0, slopes=True, window=300), id='apart_48_rows'),
     pytest.param(90, 1, 700, 6, 2, 20000, True, BF16, dict(cap=50.0, slopes=True), id='apart_wide_many_pieces'),
     pytest.param(30, 7, 1900, 14, 2, 700, True, FP16, dict(slopes=True, window=300), id='wide_few_tokens'),
     pytest.param(300, 1, 330, 16, 8, 700, True, BF16, dict(window=65), id='apart_items_in_turn'),

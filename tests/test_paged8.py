@@ -122,8 +122,9 @@ def test_shapes_that_are_refused(eight):
         ck = torch.zeros(1, 64 * 6, 2, 128, dtype=BF16)
         return paged.attention(a['q'], ck, ck.clone(), None, 0, a['table'], a['held'], Workspace(), **shape)
 
-    for shape in (dict(cap=0.0), dict(cap=-1.0), dict(cap=float('inf')), dict(cap=float('nan')), dict(window=0),
-                  dict(window=-5), dict(window=2.5), dict(slopes=torch.ones(3)), dict(slopes=torch.ones(4).double()),
+    for shape in (dict(cap=0.0), dict(cap=-1.0), dict(cap=float('inf')), dict(cap=float('nan')), dict(cap=1e5),
+                  dict(cap=1e-50), dict(window=0), dict(window=-5), dict(window=2.5), dict(window=float('inf')),
+                  dict(window=float('nan')), dict(slopes=torch.ones(3)), dict(slopes=torch.ones(4).double()),
                   dict(slopes=torch.ones(4, 1)), dict(slopes=torch.ones(8)[::2])):
         with pytest.raises(ValueError):
             call(**shape)
@@ -265,7 +266,8 @@ def test_attention_abi_rejects(eight, shaped):
                dict(tokens=1 << 30, batch=1 << 10), dict(width=1 << 26)]
     changes += BAD_CACHE if eight else [dict(ck=None), dict(cv=None), dict(kv_tok=64), dict(kv_tok=260), dict(kv_tok=1 << 24)]
     if shaped:
-        changes += [dict(cap=-1.0), dict(cap=float('nan')), dict(cap=float('inf')), dict(window=-1), dict(window=1 << 30),
+        changes += [dict(cap=-1.0), dict(cap=float('nan')), dict(cap=float('inf')), dict(cap=65537.0),
+                    dict(cap=1e-30, scale=1e20), dict(window=-1), dict(window=1 << 30),
                     dict(slopes=4098)]
     for change in changes:
         assert attention_call(eight, shaped, **change) == INVALID, change
