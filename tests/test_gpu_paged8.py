@@ -358,7 +358,7 @@ def test_attention_large(device, batch, new, held, heads, kv_heads, prefix, caus
     pytest.param([1], 3000, 4, 2, 0, id='narrow'),
     pytest.param([2] * 3, 500, 8, 2, 321, id='narrow_joint'),
 ])
-@pytest.mark.parametrize('powers', ['alike', 'rising', 'falling', 'one_page', 'one_row', 'first_page', 'wide_apart', 'tiny',
+@pytest.mark.parametrize('powers', ['alike', 'rising', 'falling', 'one_page', 'one_row', 'one_row_near', 'first_page', 'wide_apart', 'tiny',
                                     'huge', 'zeros', 'edges'])
 def test_attention_powers_of_two_of_values(device, new, held, heads, kv_heads, prefix, powers):
     """Tiles with two parts hold the values relative to the largest power of two so far
@@ -384,6 +384,8 @@ def test_attention_powers_of_two_of_values(device, new, held, heads, kv_heads, p
         e = torch.where(at[:, None] == 3, 100 + torch.arange(64, device=device), e)
     elif powers == 'one_row':                   # one that no query gives weight
         e = torch.where(place == 200, 240, e)
+    elif powers == 'one_row_near':              # and the others just within its range: fp16's smallest values
+        e = torch.where(place == 200, 139, e)
     elif powers == 'first_page':
         e = torch.where(at[:, None] == 0, torch.arange(64, device=device) * 3 + 40, e)
     elif powers == 'wide_apart':
@@ -399,7 +401,7 @@ def test_attention_powers_of_two_of_values(device, new, held, heads, kv_heads, p
         zero = live & (place % 5 == 0)[:, None]
         c.cache.v.view(torch.uint8).masked_fill_(zero[..., None], 0)
         s.masked_fill_(zero, 1)
-    if powers == 'one_row':
+    if powers.startswith('one_row'):
         page = (order + c.table[0].tolist())[200 // 64]
         # every query's score with it is about -317, others' within 16 of 0
         c.q[:] = 4.0 * (0.25 + 0.01 * c.q)
