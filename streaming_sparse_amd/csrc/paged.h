@@ -502,7 +502,11 @@ __device__ __forceinline__ void meet() {
 }
 
 // Writes what a lane holds of a row to the row's state: 16 groups of 4 dims (8 c +
-// 4 hh of row rho = j.rho0 + 32 blk + lane % 32), the maximum M and the sum l.
+// 4 hh of row rho = j.rho0 + 32 blk + lane % 32), the maximum M and the sum l.  Those of
+// wide tiles go past the L2, which would hand 17 MB of them on at the kernel's end (64 x 1
+// behind 16384, 8 bits, 42.2 -> 41.5 us; the small ones of narrow tiles do not: 4 x 1, 12
+// heads, behind 2000 11.8 and 12.2).
+template <bool PAST_L2>
 __device__ __forceinline__ void write_state(const PagedParams& p, const Job& j, const f32x16 (&O)[4], float M, float l,
                                             int blk, int lane) {
   const int rho = j.rho0 + 32 * blk + (lane & 31), hh = lane >> 5;
@@ -514,7 +518,12 @@ __device__ __forceinline__ void write_state(const PagedParams& p, const Job& j, 
   for (int c = 0; c < 16 && j.begin < j.end; ++c) {
     const f32x16& o = O[c >> 2];
     const int i = 4 * (c & 3);
-    *reinterpret_cast<f32x4*>(st + ((2 * c + hh) * 32 + col) * 4) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+    const f32x4 x{o[i], o[i + 1], o[i + 2], o[i + 3]};
+    f32x4* const to = reinterpret_cast<f32x4*>(st + ((2 * c + hh) * 32 + col) * 4);
+    if constexpr (PAST_L2)
+      __builtin_nontemporal_store(x, to);
+    else
+      *to = x;
   }
   if (hh == 0) {
     st[32 * kHeadDim + col] = M;
@@ -915,7 +924,7 @@ __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, 
   const float l = half_sum(ls);
   const float mine = m == -INFINITY ? m : m - lift;
   if constexpr (NW == 1) {
-    write_state(p, j, O, mine, l, 0, e);      // beside prefix tiles, so never the last word
+    write_state<false>(p, j, O, mine, l, 0, e);      // beside prefix tiles, so never the last word
   } else {
     // the waves' states into one: every wave hands over m, l and its 32 x 128
     // sums, [dim tile][j][lane] of 4 floats, two dim tiles at a time (8 KB a wave;
@@ -1441,7 +1450,7 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
     for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
   }
   if (j.state >= 0) {
-    write_state(p, j, O, M, l, wave, e);
+    write_state<true>(p, j, O, M, l, wave, e);
     return;
   }
   const int y = e & 31, he = e >> 5, rho = j.rho0 + 32 * wave + y;
