@@ -684,13 +684,15 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
 // which an output's 8 are all that counts (against 64 bits both 0.00166), and 8-bit
 // values are exact in fp16, but not their powers of two.  So V counts in units of 2^E,
 // one E for all pages so far (when it rises the sums follow), in which values of the
-// exponents E - 15 .. E are exact in fp16.  From the first page on that has other ones,
-// pages meet two bf16 parts in units of 1, in a loop of its own (as a branch in a wide
-// tile's first one it took its registers: 64 x 1 token behind 16384 127 us).  64 x 1
-// behind 16384 42.2 us, by two bf16 parts 46.7; 16 x 1 behind 131001 76 and 85; 64 x 1
-// behind 64, up to 2000 own rows, 33 and 36.5.  Waves by themselves, which wait for
-// their pages, keep the two parts: a second loop beside the prefix tiles' costs more
-// than it saves (4 x 1, 12 heads, behind 2000 12.7 and 11.9).
+// exponents E - 15 .. E are exact in fp16.  They take their powers themselves: in the
+// probabilities, whose smallest fp16 then holds no longer, 4096 keys of 2^-17 of the
+// largest beside values of E - 15 went missing, 3% of an output.  From the first page on
+// that has other exponents, pages meet two bf16 parts in units of 1, in a loop of its
+// own (as a branch in a wide tile's first one it took its registers: 64 x 1 token behind
+// 16384 127 us).  64 x 1 behind 16384 42.2 us, by two bf16 parts 46.7; 16 x 1 behind
+// 131001 77 and 85; 64 x 1 behind 64, up to 2000 own rows, 33 and 36.5.  Waves by
+// themselves, which wait for their pages, keep the two parts: a second loop beside the
+// prefix tiles' costs more than it saves (4 x 1, 12 heads, behind 2000 12.7 and 11.9).
 constexpr int kUnitLow = 127 - 40, kUnitHigh = 127 + 40, kUnitSpan = 15;      // as floats' exponents
 
 // A wave's walk over a tile's 8-bit pages: pages w, w + NW, ... of the list, 8 KB of K
@@ -698,11 +700,13 @@ constexpr int kUnitLow = 127 - 40, kUnitHigh = 127 + 40, kUnitSpan = 15;      //
 // neither the rows that 16 lanes read nor the transposing reads meet on a bank.
 //
 // K's powers of two go into its values on their way to 16 bits.  V's operand holds
-// eight rows of one dim, so the powers go into the probabilities, p v = (p 2^e)
-// (v / 2^e), which, but for RELATIVE pages, meet V in bf16 whatever the queries' type:
-// its range holds every power of two and two parts carry more bits than an fp16 output.  Score S[i] is key 16
-// (i / 8) + 8 hh + i % 8 of its half page (the K operand's rows are taken in that
-// order), so that a lane's probabilities belong to the eight rows of an operand.
+// eight rows of one dim, so its powers go into the probabilities, p v = (p 2^e) (v /
+// 2^e), which meet V in bf16 whatever the queries' type: its range holds every power of
+// two and two parts carry more bits than an fp16 output.  On RELATIVE pages they go into
+// V all the same, by a product a pair of rows, which costs 1% (16 x 1 behind 131001 76.5
+// and 77.4 us).  Score S[i] is key 16 (i / 8) + 8 hh + i % 8 of its half page (the K
+// operand's rows are taken in that order), so that a lane's probabilities belong to the
+// eight rows of an operand.
 constexpr int kWave8 = 2 * kPage * kHeadDim + 512;     // K, V, the exponents as they come, V's as floats
 __device__ __forceinline__ int swz8(int row) { return (row & 6) | ((row >> 3) & 1); }
 
@@ -712,6 +716,7 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
   constexpr bool F16 = How::F16, SHAPED = How::SHAPED, RELATIVE = !F16 && NW > 1;
   typedef __attribute__((address_space(3))) float lds_f32;
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+  typedef __attribute__((address_space(3))) _Float16 lds_f16;
   const int r = lane & 31, hh = lane >> 5;
   u32x4 qop[8];
   Sight x;
@@ -740,6 +745,7 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
   lds_u8* const vb = kb + kPage * kHeadDim;
   lds_u8* const raw = vb + kPage * kHeadDim;
   lds_f32* const vscale = (lds_f32*)(raw + 256);
+  lds_f16* const vfactor = (lds_f16*)vscale;
   auto issue = [&](const uint8_t* from, const Unit& u, lds_u8* to) {
     // an absent page reads page 0: its rows are masked and its values cleared
     const uint8_t* const at = scalar(from + max(u.page, 0) * p.kv_tok);
@@ -802,7 +808,11 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
         for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
       }
       unit = to;
-      vscale[lane] = seen ? exponent(e + 127 - to) : 0.0f;
+      const float f = seen ? exponent(e + 127 - to) : 0.0f;
+      if constexpr (fine)
+        vfactor[lane] = (_Float16)f;
+      else
+        vscale[lane] = f;
     } else {
       vscale[lane] = seen ? exponent(raw[kPage + lane]) : 0.0f;
     }
@@ -853,17 +863,19 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
     }
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      // the probabilities of keys 16 ks + 8 hh .. + 7, in two parts
-      u32x4 hi, lo;
+      // the probabilities of keys 16 ks + 8 hh .. + 7, in two parts, or in one beside values
+      // times their rows' powers
+      u32x4 hi, lo, factor;
+      if constexpr (fine) factor = *(lds_u32x4*)(vfactor + 16 * ks + 8 * hh);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const f32x4 f = *(lds_f32x4*)(vscale + 16 * ks + 8 * hh + 4 * half);
         const f32x16& P = S[ks >> 1];
         const int i = 8 * (ks & 1) + 4 * half;
         if constexpr (fine) {
-          hi[2 * half] = pack2<true>(P[i] * f[0], P[i + 1] * f[1]);
-          hi[2 * half + 1] = pack2<true>(P[i + 2] * f[2], P[i + 3] * f[3]);
+          hi[2 * half] = pack2<true>(P[i], P[i + 1]);
+          hi[2 * half + 1] = pack2<true>(P[i + 2], P[i + 3]);
         } else {
+          const f32x4 f = *(lds_f32x4*)(vscale + 16 * ks + 8 * hh + 4 * half);
           const u32x2 a = split2<false>(P[i] * f[0], P[i + 1] * f[1]), b = split2<false>(P[i + 2] * f[2], P[i + 3] * f[3]);
           hi[2 * half] = a[0];
           hi[2 * half + 1] = b[0];
@@ -876,7 +888,9 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
         // dim 32 dt + lane % 32 of the same keys
         const int g = lane >> 4, i = lane & 15, row = 16 * ks + 8 * (g >> 1) + (i >> 1);
         const u32x2 w = tr8(vb + row * 128 + (((2 * dt + (g & 1)) ^ swz8(row)) << 4) + (i & 1) * 8);
-        const u32x4 va = widen<fine>(w[0], w[1], 1.0f);
+        u32x4 va = widen<fine>(w[0], w[1], 1.0f);
+        if constexpr (fine)
+          va = __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, va) * __builtin_bit_cast(f16x8, factor));
         O[dt] = mma<fine>(va, hi, O[dt]);
         if constexpr (!fine) O[dt] = mma<false>(va, lo, O[dt]);
       }
