@@ -25,7 +25,8 @@ extern "C" {
  * key's or value's row is rounded to its 16-bit type as there; its power of two is
  * the smallest 2^e, e >= -126, with max |x| <= 448 * 2^e over its finite elements,
  * and x 2^-e is rounded to e4m3 (nearest, ties to even).  Infinities and NaN become
- * NaN; fp16 elements from 63488 on are held as 61440. */
+ * NaN; fp16 elements from 63488 on are held as 61440, bf16 ones from 1.9375 * 2^127 on as
+ * 1.875 * 2^127, so that what is finite stays so. */
 int ssa_paged8_append(const void* q, long long q_token_stride, long long q_head_stride, void* q_out,
                       long long out_token_stride, long long out_head_stride, const void* k, long long k_token_stride,
                       long long k_head_stride, const void* v, long long v_token_stride, long long v_head_stride,

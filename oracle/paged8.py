@@ -24,8 +24,9 @@ def quantise(x, s=None):
     grid, which times 2^(s - 127) are what the rows stand for."""
     s = exponents(x) if s is None else s
     y, finite = x.double(), torch.isfinite(x)
-    if x.dtype is torch.float16:
-        y = torch.where(y.abs() >= 63488, torch.copysign(torch.full_like(y, 61440.0), y), y)
+    # rounded up, these would be infinite in their 16-bit type
+    last = 2.0 ** (15 if x.dtype is torch.float16 else 127)
+    y = torch.where(y.abs() >= 1.9375 * last, torch.copysign(torch.full_like(y, 1.875 * last), y), y)
     y = torch.where(finite, y, 0.0) * torch.exp2((127 - s).double())[..., None]
     step = torch.exp2(torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -6))) - 3)
     y = torch.round(y / step) * step    # half to even

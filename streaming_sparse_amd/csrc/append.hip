@@ -129,20 +129,20 @@ typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // The 8 values that a lane holds of a row (16 lanes) in 8 bits, and the row's biased
-// exponent.  Infinities and NaN become NaN and count nothing for the exponent; fp16 values
-// that would be rounded to 65536, which fp16 does not hold, become 61440.
+// exponent.  Infinities and NaN become NaN and count nothing for the exponent; values that
+// would be rounded to the power of two behind the type's largest, fp16's to 65536 and
+// bf16's to 2^128, become 15 / 16 of it.
 template <bool F16>
 __device__ __forceinline__ u32x2 quantise(u32x4 x, uint32_t* exponent) {
   // magnitudes, moved up so that those of infinities and NaN are negative
   constexpr uint16_t kUp = F16 ? 0x0400 : 0x0080;
+  constexpr int16_t kLargest = (F16 ? 0x7bbf : 0x7f77) + kUp;      // of those that are not rounded up
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     i16x2 m = __builtin_bit_cast(i16x2, (u16x2)(__builtin_bit_cast(u16x2, x[e] & 0x7fff7fffu) + (u16x2){kUp, kUp}));
-    if constexpr (F16) {
-      m = __builtin_elementwise_min(m, (i16x2){0x7bbf + 0x400, 0x7bbf + 0x400});
-      x[e] = (x[e] & 0x80008000u) | __builtin_bit_cast(uint32_t, (u16x2)(__builtin_bit_cast(u16x2, m) - (u16x2){kUp, kUp}));
-    }
+    m = __builtin_elementwise_min(m, (i16x2){kLargest, kLargest});
+    x[e] = (x[e] & 0x80008000u) | __builtin_bit_cast(uint32_t, (u16x2)(__builtin_bit_cast(u16x2, m) - (u16x2){kUp, kUp}));
     top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(m, __builtin_bit_cast(i16x2, top)));
   }
   int most = max((int)(int16_t)top, (int)(int16_t)(top >> 16));

@@ -70,7 +70,8 @@ def append(k, v, cache, table, held, *, q=None, q_out=None, starts=None, freqs=N
     """``paged.append`` into an 8-bit cache: keys and values are rotated and rounded
     to their 16-bit type as there, then quantised.  Infinities and NaN are held as
     NaN and do not count for their row's power of two; fp16 elements from 63488
-    on are held as 61440.  Queries stay in 16 bits."""
+    on are held as 61440, bf16 ones from 1.9375 * 2^127 on as 1.875 * 2^127.
+    Queries stay in 16 bits."""
     code = _TYPES.get(k.dtype)
     if code is None:
         raise TypeError("k must be bfloat16 or float16")
