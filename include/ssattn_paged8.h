@@ -22,8 +22,8 @@ extern "C" {
 #endif
 
 /* ssa_paged_append into an 8-bit cache, of whose rows the strides are above.  A
- * key's or value's row is rounded to its 16-bit type as there; its power of two is
- * the smallest 2^e, e >= -126, with max |x| <= 448 * 2^e over its finite elements,
+ * key's or value's row is rounded to its 16-bit type as there (keys turn in float64 and
+ * are rounded to float32 first); its power of two is the smallest 2^e, e >= -126, with max |x| <= 448 * 2^e over its finite elements,
  * and x 2^-e is rounded to e4m3 (nearest, ties to even).  Infinities and NaN become
  * NaN; fp16 elements from 63488 on are held as 61440, bf16 ones from 1.9375 * 2^127 on as
  * 1.875 * 2^127, so that what is finite stays so. */

@@ -98,6 +98,14 @@ __device__ __forceinline__ void turn64(double h, double* sine, double* cosine) {
   *cosine = (q + 1) & 2 ? -b : b;
 }
 
+// x in float32 (the empty asm keeps the compiler from rounding it to 16 bits at once, a
+// longer sequence with another result where x lies next to a border).
+__device__ __forceinline__ float single(double x) {
+  float y = (float)x;
+  asm volatile("" : "+v"(y));
+  return y;
+}
+
 // The sequence and place of packed token t among sequences that start at starts[0..] (null:
 // per_seq tokens each); false: behind the last one.
 __device__ __forceinline__ bool place_of(const int32_t* starts, int batch, int per_seq, int t, int lane, int* b,
@@ -306,11 +314,11 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(AppendParams p) {
             const double a = lo_of<F16>(x[u][e]), d = hi_of<F16>(x[u][e]);
             uint32_t w;
             if constexpr (INTERLEAVED) {
-              w = pack<F16>((float)(a * C64[e] - d * S64[e]), (float)(a * S64[e] + d * C64[e]));
+              w = pack<F16>(single(a * C64[e] - d * S64[e]), single(a * S64[e] + d * C64[e]));
             } else {
               const uint32_t o = (uint32_t)__builtin_amdgcn_ds_bpermute(partner << 2, (int)x[u][e]);
-              w = pack<F16>((float)(a * C64[2 * e] - lo_of<F16>(o) * S64[2 * e]),
-                            (float)(d * C64[2 * e + 1] - hi_of<F16>(o) * S64[2 * e + 1]));
+              w = pack<F16>(single(a * C64[2 * e] - lo_of<F16>(o) * S64[2 * e]),
+                            single(d * C64[2 * e + 1] - hi_of<F16>(o) * S64[2 * e + 1]));
             }
             y[e] = is_key && (INTERLEAVED ? e < turning : turning > 0) ? w : y[e];
           }

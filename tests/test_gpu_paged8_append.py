@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from oracle import paged as plain
 from oracle import paged8 as oracle
 from streaming_sparse_amd import paged8
 
@@ -53,3 +54,25 @@ def test_finite_values_stay_finite(device, dtype):
         want, s = oracle.quantise(given)
         # fp16 rounds those below its smallest normal value
         assert torch.equal(got, oracle.values(want, s).to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('interleaved', [True, False], ids=['pairs', 'halves'])
+@pytest.mark.parametrize('dtype', [BF16, FP16], ids=['bf16', 'fp16'])
+def test_keys_turn_in_float64(device, dtype, interleaved):
+    """16 million elements of turned keys as float64 has them, rounded to float32, to 16 bits and to 8: bit for bit.
+    Angles of up to 8192 radians are off by 2^-40, which brings an element to another 16-bit value with a chance of
+    2^-40 / 2^-12 at most; a turn in float32 does so to an 8-bit value of every 10^5, leaving out the rounding to
+    float32 to one of every 2 x 10^6."""
+    n, g = 8192, 16
+    gen = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(n, g, 128, generator=gen).to(dtype) for _ in range(2))
+    freqs = 10000.0 ** (-torch.arange(64, dtype=torch.float64) / 64)
+    turned = plain.rotate(k.double(), torch.arange(n)[:, None], freqs, (64,), interleaved).float().to(dtype)
+    cache, got_k, got_v = one_sequence(device, k.to(device), v.to(device), dtype, freqs=freqs.to(device),
+                                       interleaved=interleaved)
+    for got, given in ((got_k, turned), (got_v, v)):
+        want, s = oracle.quantise(given.to(device))
+        want = oracle.values(want, s).to(dtype)
+        off = int((got != want).sum())
+        assert off == 0, off
