@@ -40,10 +40,11 @@ constexpr int kPage = 64;
 constexpr int kMostRows = (1 << 30) - 1;       // of a sequence, and of a window
 
 // What a kernel is made for: fp16 rows (else bf16), a cache of 8-bit rows (else of
-// 16-bit ones in the queries' type), shaped scores (else plain ones).
-template <bool F16_, bool Q8_, bool SHAPED_>
+// 16-bit ones in the queries' type), shaped scores (else plain ones), two parts of a
+// probability as such (else one of fp16 may stand for two of bf16 over 8-bit rows).
+template <bool F16_, bool Q8_, bool SHAPED_, bool BOTH_ = false>
 struct Mode {
-  static constexpr bool F16 = F16_, Q8 = Q8_, SHAPED = SHAPED_;
+  static constexpr bool F16 = F16_, Q8 = Q8_, SHAPED = SHAPED_, BOTH = BOTH_;
 };
 
 struct PagedParams {
@@ -687,7 +688,7 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
 // exponents E - 15 .. E are exact in fp16.  They take their powers themselves: in the
 // probabilities, whose smallest fp16 then holds no longer, 4096 keys of 2^-17 of the
 // largest beside values of E - 15 went missing, 3% of an output.  From the first page on
-// that has other exponents, pages meet two bf16 parts in units of 1, in a loop of its
+// that has other exponents pages meet two bf16 parts in units of 1, in a loop of its
 // own (as a branch in a wide tile's first one it took its registers: 64 x 1 token behind
 // 16384 127 us).  64 x 1 behind 16384 42.2 us, by two bf16 parts 46.7; 16 x 1 behind
 // 131001 77 and 85; 64 x 1 behind 64, up to 2000 own rows, 33 and 36.5.  Waves by
@@ -703,8 +704,8 @@ constexpr int kUnitLow = 127 - 40, kUnitHigh = 127 + 40, kUnitSpan = 15;      //
 // eight rows of one dim, so its powers go into the probabilities, p v = (p 2^e) (v /
 // 2^e), which meet V in bf16 whatever the queries' type: its range holds every power of
 // two and two parts carry more bits than an fp16 output.  On RELATIVE pages they go into
-// V all the same, by a product a pair of rows, which costs 1% (16 x 1 behind 131001 76.5
-// and 77.4 us).  Score S[i] is key 16 (i / 8) + 8 hh + i % 8 of its half page (the K
+// V all the same, by a product a pair of rows, which costs 1 to 2% (16 x 1 behind 131001
+// 71.4 and 73.0 us).  Score S[i] is key 16 (i / 8) + 8 hh + i % 8 of its half page (the K
 // operand's rows are taken in that order), so that a lane's probabilities belong to the
 // eight rows of an operand.
 constexpr int kWave8 = 2 * kPage * kHeadDim + 512;     // K, V, the exponents as they come, V's as floats
@@ -713,7 +714,7 @@ __device__ __forceinline__ int swz8(int row) { return (row & 6) | ((row >> 3) & 
 template <class How, int NW>
 __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave,
                                       f32x16 (&O)[4], float& m, float& ls) {
-  constexpr bool F16 = How::F16, SHAPED = How::SHAPED, RELATIVE = !F16 && NW > 1;
+  constexpr bool F16 = How::F16, SHAPED = How::SHAPED, RELATIVE = !F16 && !How::BOTH && NW > 1;
   typedef __attribute__((address_space(3))) float lds_f32;
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
   typedef __attribute__((address_space(3))) _Float16 lds_f16;
@@ -922,7 +923,7 @@ constexpr int kWaveBytes = How::Q8 ? kWave8 : 2 * kHalf;      // a narrow wave's
 template <class How, int NW>
 __device__ __forceinline__ void narrow_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
   constexpr bool F16 = How::F16;
-  constexpr float lift = kLift<How::Q8 ? !F16 && NW != 1 : F16>;
+  constexpr float lift = kLift<How::Q8 ? !F16 && !How::BOTH && NW != 1 : F16>;
   f32x16 O[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
@@ -1095,7 +1096,7 @@ struct Staged {
 
 template <class How, bool PAIRS, bool TWO>
 __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, lds_u8* ring, int lane, int wave) {
-  constexpr bool F16 = How::F16, Q8 = How::Q8, SHAPED = How::SHAPED, RELATIVE = Q8 && !F16 && TWO,
+  constexpr bool F16 = How::F16, Q8 = How::Q8, SHAPED = How::SHAPED, RELATIVE = Q8 && !F16 && !How::BOTH && TWO,
                  V16 = F16 || RELATIVE;
   constexpr int kSlots = kRing<PAIRS>;
   const int r = lane & 31, hh = lane >> 5;
@@ -2033,6 +2034,8 @@ int run(PagedParams p, Sizes z, float scale, int flags, void* workspace, long lo
     auto join = [&](auto kernel) { launch(kernel, joins, 64 * kJoinWaves); };
     if (!plan.wide())
       plan.apart() ? start(narrow_kernel<How, true>) : start(narrow_kernel<How, false>);
+    else if constexpr (How::BOTH)
+      plan.apart() ? start(wide_kernel<How, true, false, true>) : start(wide_kernel<How, false, false, true>);
     else if (plan.apart())
       two ? start(wide_kernel<How, true, false, true>) : start(wide_kernel<How, true, false, false>);
     else if (plan.pairs) {
@@ -2045,7 +2048,12 @@ int run(PagedParams p, Sizes z, float scale, int flags, void* workspace, long lo
     else
       plan.many() ? join(join_kernel<How, false, true>) : join(join_kernel<How, false, false>);
   };
-  (flags & 1) ? with(Mode<true, Q8, SHAPED>{}) : with(Mode<false, Q8, SHAPED>{});
+  if (flags & 1)
+    with(Mode<true, Q8, SHAPED>{});
+  else if (Q8 && parts == 2)
+    with(Mode<false, Q8, SHAPED, Q8>{});
+  else
+    with(Mode<false, Q8, SHAPED>{});
   return (int)hipGetLastError();
 }
 

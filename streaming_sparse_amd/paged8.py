@@ -130,8 +130,9 @@ def attention(q, cache, prefix, prefix_tokens, table, lengths, workspace, *, sta
     16-bit one: the same numbers as attention over the rows that `read` returns, up
     to the roundings named there.  q bf16 or fp16, of the type whose rows were
     appended.  Tiles of up to 32 rows take probabilities in two parts; with bf16
-    queries one fp16 part may stand for two.  Sums reach 2^15 times the values' size
-    times the rows: values from 2^90 on may come out infinite."""
+    queries one fp16 part (11 bits) may stand for two, but for single_av=False.
+    Sums reach 2^15 times the values' size times the rows: values from 2^90 on may
+    come out infinite."""
     code = _TYPES.get(q.dtype)
     if code is None:
         raise TypeError("q must be bfloat16 or float16")

@@ -54,3 +54,45 @@ def test_many_small_probabilities_keep_their_weight(device, batch, new, single, 
     far = (out.double().unflatten(0, (batch, new)) - want).abs() / spread
     limit = torch.finfo(BF16).eps / 2 + 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -20
     assert float(far.max()) <= limit, (float(far.max()), limit)
+
+
+@pytest.mark.parametrize('how', [dict(), dict(window=1 << 20)], ids=['plain', 'shaped'])
+@pytest.mark.parametrize('batch,new,prefix,held', [
+    pytest.param(64, 1, 0, 5, id='narrow'),
+    pytest.param(1, 100, 0, 6, id='wide'),
+    pytest.param(90, 1, 1500, 3, id='apart'),
+])
+def test_two_parts_that_are_asked_for(device, batch, new, prefix, held, how):
+    """single_av=False: how many outputs are not the float64 result's rounding.  With all values of one sign an error e of
+    an output, relative, takes |e| / step of them, step 2^-7 to 2^-8, to the other side of a border: of a few keys whose
+    probabilities are off by 2^-16 / sqrt(12) each (two parts of 8 bits), scores by 2^-18 and exponentials by 2^-20,
+    0.8 * 2^-17 / 2^-7.5, one in 900.  One fp16 part is off by 2^-10 / sqrt(12), the root of the sum of the squared
+    probabilities of a few keys a half of that: one in 50.  At most one in 256 is allowed."""
+    G, H = 8, 32
+    width, shared = 2, -(-prefix // 64)
+    pages = shared + batch * width
+    g = torch.Generator(device=device).manual_seed(2)
+    cache = paged8.Cache.empty(pages, G, device)
+    v = 256 + 192 * torch.rand(pages, G, 64, 128, generator=g, device=device)
+    cache.v.copy_(v.to(torch.float8_e4m3fn))
+    k = torch.randn(pages, G, 64, 128, generator=g, device=device)
+    k *= 64.0
+    if shared:                            # all but two keys of the prefix's first two pages score about -40
+        none = torch.ones(shared, 1, 64, 1, dtype=torch.bool, device=device)
+        none[:2, :, 7:9] = False
+        k[:shared, ..., :4] = torch.where(none, -448.0, k[:shared, ..., :4])
+    cache.k.copy_(k.clamp(-448, 448).to(torch.float8_e4m3fn))
+    cache.scales[:, :, 0] = 121
+    cache.scales[:, :, 1] = torch.randint(116, 122, (pages, G, 64), generator=g, device=device).to(torch.uint8)
+    q = torch.randn(batch * new, H, 128, generator=g, device=device).to(BF16)
+    if shared:
+        q[..., :4] = 16.0
+    order = torch.arange(pages, dtype=torch.int32, device=device)
+    table = order[shared:].reshape(batch, width).contiguous()
+    lengths = ints([held] * batch, device)
+    starts = torch.arange(batch + 1, device=device) * new
+    out = paged8.attention(q, cache, order[:shared].contiguous(), prefix, table, lengths, Workspace(), causal=False,
+                           single_av=False, **how)
+    want, _, _ = oracle.attention(q, *oracle.pages8(cache), order[:shared], prefix, table, lengths, starts, causal=False)
+    off = float((out != want.float().to(BF16)).double().mean())
+    assert off <= 2.0 ** -8, off
