@@ -31,6 +31,7 @@ class Cache:
     k: torch.Tensor          # [P, G, 64, 128] float8_e4m3fn
     v: torch.Tensor
     scales: torch.Tensor     # [P, G, 2, 64] uint8
+    bf16: bool = False       # whether rows were appended as bfloat16, of which fp16 may not hold the values
 
     @classmethod
     def empty(cls, pages, kv_heads, device):
@@ -78,8 +79,11 @@ def append(k, v, cache, table, held, *, q=None, q_out=None, starts=None, freqs=N
     if not -_FAR <= first <= _FAR:
         raise ValueError("first must lie within 2^53")
     pages, g, where = _cache(cache, k.get_device())
-    return _append("ssa_paged8_append", where, pages, g, k, v, table, held, q, q_out, starts, freqs, axes, positions,
-                   first, interleaved, workspace, code)
+    q = _append("ssa_paged8_append", where, pages, g, k, v, table, held, q, q_out, starts, freqs, axes, positions,
+                first, interleaved, workspace, code)
+    if not code:
+        cache.bf16 = True
+    return q
 
 
 def read(cache, table, first, tokens, *, starts=None, dtype=torch.bfloat16, k_out=None, v_out=None, workspace=None):
@@ -129,13 +133,17 @@ def attention(q, cache, prefix, prefix_tokens, table, lengths, workspace, *, sta
     """``paged.attention`` over an 8-bit cache, its arguments and results those of the
     16-bit one: the same numbers as attention over the rows that `read` returns, up
     to the roundings named there.  q bf16 or fp16, of the type whose rows were
-    appended.  Tiles of up to 32 rows take probabilities in two parts; with bf16
+    appended: fp16 queries are refused where `append` has put bf16 rows through this
+    Cache, whose values fp16 need not hold (one made over filled tensors does not
+    know).  Tiles of up to 32 rows take probabilities in two parts; with bf16
     queries one fp16 part (11 bits) may stand for two, but for single_av=False.
     Sums reach 2^15 times the values' size times the rows: values from 2^90 on may
     come out infinite."""
     code = _TYPES.get(q.dtype)
     if code is None:
         raise TypeError("q must be bfloat16 or float16")
+    if code and cache.bf16:
+        raise TypeError("float16 queries over rows that were appended as bfloat16")
     pages, g, where = _cache(cache, q.get_device())
     return _attend("ssa_paged8_attention", True, where, pages, g, q, prefix, prefix_tokens, table, lengths, workspace,
                    starts, causal, scale, want_lse, out, single_av, cap, slopes, window, code)

@@ -181,6 +181,29 @@ def test_read_keeps_two_buffers_of_a_workspace(no_launch):
     assert len(ws.entries) == 4
 
 
+def test_half_queries_over_bfloat16_rows_are_refused(no_launch):
+    """fp16 does not hold every value of rows appended as bf16; bf16 holds all of those appended as fp16."""
+    a, b = args(), args(dtype=torch.float16)
+
+    def attend(x, cache, **more):
+        paged8.attention(x['q'], cache, None, 0, x['table'], x['held'], Workspace(), **more)
+
+    cache = a['cache']
+    attend(a, cache), attend(b, cache)                        # nothing is known of its rows
+    paged8.append(b['k'], b['v'], cache, b['table'], b['held'])
+    attend(a, cache), attend(b, cache)
+    paged8.append(a['k'], a['v'], cache, a['table'], a['held'])
+    calls = len(no_launch)
+    for more in (dict(), dict(cap=5.0)):
+        with pytest.raises(TypeError):
+            attend(b, cache, **more)
+    assert len(no_launch) == calls
+    attend(a, cache)
+    paged8.append(b['k'], b['v'], cache, b['table'], b['held'])
+    with pytest.raises(TypeError):
+        attend(b, cache)
+
+
 def test_sources_keep_nan_semantics():
     for source in ("paged_shaped.hip", "paged8.hip", "paged8_shaped.hip"):
         flags = build.FLAGS + build.EXTRA.get(source, [])
