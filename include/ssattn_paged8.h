@@ -52,7 +52,8 @@ int ssa_paged8_read(const void* cache_k, const void* cache_v, long long kv_page_
  * meets V in two parts, whatever the flags.  Where there are two, the queries are bf16
  * and the flags do not ask for two, they may be one of fp16 instead, which carries 11
  * bits down to 2^-21 of a row's largest probability (values whose powers of two lie
- * within 2^15 of the largest of the pages walked before). */
+ * within 2^15 of the largest of the pages walked before; rows whose byte is 1, values
+ * below 2^-117, count as zeros then). */
 int ssa_paged8_attention(const void* q, long long q_token_stride, long long q_head_stride, const void* cache_k,
                          const void* cache_v, long long kv_page_stride, long long kv_head_stride, const void* scales,
                          long long scales_page_stride, long long scales_head_stride, const int32_t* prefix,

@@ -685,7 +685,8 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
 // which an output's 8 are all that counts (against 64 bits both 0.00166), and 8-bit
 // values are exact in fp16, but not their powers of two.  So V counts in units of 2^E,
 // one E for all pages so far (when it rises the sums follow), in which values of the
-// exponents E - 15 .. E are exact in fp16.  They take their powers themselves: in the
+// exponents E - 15 .. E are exact in fp16, and so are zeros: rows of the least exponent
+// count as such (what they may hold is below 2^-117).  Values take their powers themselves: in the
 // probabilities, whose smallest fp16 then holds no longer, 4096 keys of 2^-17 of the
 // largest beside values of E - 15 went missing, 3% of an output.  From the first page on
 // that has other exponents pages meet two bf16 parts in units of 1, in a loop of its
@@ -801,7 +802,7 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
       if constexpr (fine) {
         for (uint64_t up; to < kUnitHigh && (up = __ballot(seen && e > to));)
           to = min(__builtin_amdgcn_readlane(e, __builtin_ctzll(up)), kUnitHigh);
-        if (__builtin_expect(__ballot(seen && (e > to || e < to - kUnitSpan)) != 0, 0)) return false;
+        if (__builtin_expect(__ballot(seen && (e > to || (e < to - kUnitSpan && e > 1))) != 0, 0)) return false;
       }
       if (to != unit && unit > 0) {
         const float a = __uint_as_float((uint32_t)(127 + unit - to) << 23);
@@ -809,7 +810,7 @@ __device__ __forceinline__ void walk8(const PagedParams& p, const Job& j, lds_u8
         for (int dt = 0; dt < 4; ++dt) O[dt] *= a;
       }
       unit = to;
-      const float f = seen ? exponent(e + 127 - to) : 0.0f;
+      const float f = seen && !(fine && e == 1) ? exponent(e + 127 - to) : 0.0f;
       if constexpr (fine)
         vfactor[lane] = (_Float16)f;
       else
@@ -1183,13 +1184,14 @@ __device__ __forceinline__ void wide_tile(const PagedParams& p, const Job& j, ld
       if (u < fine_end) {
         for (uint64_t more; unit < kUnitHigh && (more = __ballot(seen && e > unit));)
           unit = min(__builtin_amdgcn_readlane(e, __builtin_ctzll(more)), kUnitHigh);
-        if (__ballot(seen && (e > unit || e < unit - kUnitSpan))) fine_end = u;
+        if (__ballot(seen && (e > unit || (e < unit - kUnitSpan && e > 1)))) fine_end = u;
       }
       if (u >= fine_end) unit = 127;
     }
     lds_u8* const kt = kring + slot * kTile + row * 256;
     lds_u8* const vt = vring + slot * kTile + row * 256;
-    const float ks = __uint_as_float(from.ks << 23), vs = __uint_as_float((RELATIVE ? from.vs + 127 - unit : from.vs) << 23);
+    const float ks = __uint_as_float(from.ks << 23);
+    const float vs = __uint_as_float((RELATIVE ? (uint32_t)max((int)from.vs + 127 - unit, 1) : from.vs) << 23);
     *(lds_u32x4*)(kt + ((c ^ (row & 15)) << 4)) = widen<F16>(from.k[0], from.k[1], ks);
     *(lds_u32x4*)(kt + (((c + 1) ^ (row & 15)) << 4)) = widen<F16>(from.k[2], from.k[3], ks);
     u32x4 a, b;

@@ -96,3 +96,45 @@ def test_two_parts_that_are_asked_for(device, batch, new, prefix, held, how):
     want, _, _ = oracle.attention(q, *oracle.pages8(cache), order[:shared], prefix, table, lengths, starts, causal=False)
     off = float((out != want.float().to(BF16)).double().mean())
     assert off <= 2.0 ** -8, off
+
+
+WAYS = [
+    # batch, new tokens, prefix, held
+    pytest.param(64, 1, 0, 700, id='narrow'),
+    pytest.param(90, 1, 1500, 70, id='apart'),
+    pytest.param(8, 1, 3000, 70, id='narrow_apart'),
+]
+
+
+def case(device, batch, new, prefix, held, G=8, H=32):
+    width, shared = -(-(held + new) // 64), -(-prefix // 64)
+    pages = shared + batch * width
+    g = torch.Generator(device=device).manual_seed(5)
+    cache = paged8.Cache.empty(pages, G, device)
+    for x in (cache.k, cache.v):
+        x.copy_((100 * torch.randn(pages, G, 64, 128, generator=g, device=device)).clamp(-448, 448).to(torch.float8_e4m3fn))
+    cache.scales.fill_(120)
+    q = torch.randn(batch * new, H, 128, generator=g, device=device).to(BF16)
+    order = torch.arange(pages, dtype=torch.int32, device=device)
+    return cache, (q, cache, order[:shared].contiguous(), prefix, order[shared:].reshape(batch, width).contiguous(),
+                   ints([held + new] * batch, device))
+
+
+@pytest.mark.parametrize('how', [dict(), dict(window=1 << 20)], ids=['plain', 'shaped'])
+@pytest.mark.parametrize('batch,new,prefix,held', WAYS)
+def test_zero_rows_cost_no_part(device, batch, new, prefix, held, how):
+    """A value row of zeros has the least power of two; the same outputs, bit for bit, as with its neighbours' power.
+    One of NaN has it too, and shows."""
+    cache, a = case(device, batch, new, prefix, held)
+    cache.v.view(torch.uint8)[:, :, 5] = 0
+    cache.v.view(torch.uint8)[::3, :, 11] = 0x80
+    want = paged8.attention(*a, Workspace(), **how)
+    cache.scales[:, :, 1, 5] = 1
+    cache.scales[::3, :, 1, 11] = 1
+    assert torch.equal(paged8.attention(*a, Workspace(), **how), want)
+    exact = paged8.attention(*a, Workspace(), single_av=False, **how)
+    assert not torch.equal(exact, want)              # so the comparison above tells one part from two
+    page = int(a[4][0, 0])
+    cache.v.view(torch.uint8)[page, 0, 5, 3] = 0x7f
+    got = paged8.attention(*a, Workspace(), **how)
+    assert torch.isnan(got[0, :4, 3]).all() and torch.isfinite(got[0, :4, 4:]).all() and torch.isfinite(got[1:]).all()
