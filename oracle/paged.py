@@ -97,15 +97,16 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, starts
 
 
 
-def error_limit(want, p2, p2v2, dtype, parts):
+def error_limit(want, p2, p2v2, dtype, parts, part=None):
     """What the root of the summed squared errors of outputs `want` [..., 128] may
     be, given sum p^2 [...] and sum p^2 v^2 [..., 128] over their normalised
-    probabilities, each of which meets V in `parts` 16-bit parts.
+    probabilities, each of which meets V in `parts` 16-bit parts, one of which is of
+    type `part` (else of the outputs').
 
     * A result rounded once is off by an error uniform within half a step: mean
       square step^2 / 12, the sum's standard deviation sqrt(4 / 5) of the root of
       the squared means' sum.  Six of those are allowed, here and below.
-    * One part: a probability is off by at most eps / 2 of itself, mean square
+    * One part: a probability is off by at most eps / 2 of itself (the part's), mean square
       below eps^2 / 12, one error for all 128 dims: their quadratic form over a row
       has the mean eps^2 / 12 sum p^2 v^2 and a variance of at most twice its square
       times 1 / 128 + sum p^2.
@@ -119,6 +120,6 @@ def error_limit(want, p2, p2v2, dtype, parts):
     e = step * step / 12
     limit = (e.sum() + 6 * (0.8 * (e * e).sum()).sqrt()).sqrt()
     if parts == 1:
-        e = p2v2.sum(-1) * info.eps ** 2 / 12
+        e = p2v2.sum(-1) * torch.finfo(part or dtype).eps ** 2 / 12
         limit = limit + (e.sum() + 6 * (2 * (e * e * (1 / 128 + p2)).sum()).sqrt()).sqrt()
     return limit + 2.0 ** -15 * (p2v2.sum() + (want * want).sum()).sqrt()

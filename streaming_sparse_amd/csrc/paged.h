@@ -686,14 +686,14 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
 // values are exact in fp16, but not their powers of two.  So V counts in units of 2^E,
 // one E for all pages so far (when it rises the sums follow), in which values of the
 // exponents E - 15 .. E are exact in fp16, and so are zeros: rows of the least exponent
-// count as such (what they may hold is below 2^-117).  Values take their powers themselves: in the
-// probabilities, whose smallest fp16 then holds no longer, 4096 keys of 2^-17 of the
-// largest beside values of E - 15 went missing, 3% of an output.  From the first page on
-// that has other exponents pages meet two bf16 parts in units of 1, in a loop of its
-// own (as a branch in a wide tile's first one it took its registers: 64 x 1 token behind
-// 16384 127 us).  64 x 1 behind 16384 42.2 us, by two bf16 parts 46.7; 16 x 1 behind
-// 131001 77 and 85; 64 x 1 behind 64, up to 2000 own rows, 33 and 36.5.  Waves by
-// themselves, which wait for their pages, keep the two parts: a second loop beside the
+// count as such (what they may hold is below 2^-117).  Values take their powers
+// themselves: in the probabilities, whose smallest fp16 then holds no longer, 4096 keys
+// of 2^-17 of the largest beside values of E - 15 went missing, 3% of an output.  From
+// the first page on that has other exponents pages meet two bf16 parts in units of 1, in
+// a loop of its own (as a branch in a wide tile's first one it took its registers: 64 x 1
+// token behind 16384 127 us).  64 x 1 behind 16384 42.2 us, by two bf16 parts 46.7; 16 x
+// 1 behind 131001 77 and 85; 64 x 1 behind 64, up to 2000 own rows, 33 and 36.5.  Waves
+// by themselves, which wait for their pages, keep the two parts: a second loop beside the
 // prefix tiles' costs more than it saves (4 x 1, 12 heads, behind 2000 12.7 and 11.9).
 constexpr int kUnitLow = 127 - 40, kUnitHigh = 127 + 40, kUnitSpan = 15;      // as floats' exponents
 
