@@ -9,7 +9,8 @@
  * 16), their biased exponents, 64 of the keys and then 64 of the values, at byte
  * P * scales_page_stride + h * scales_head_stride of `scales` (4-byte aligned,
  * strides multiples of 4).  A value x with its row's byte s (1..254) stands for x
- * 2^(s - 127).  bf16 holds every such value; fp16 those of rows appended as fp16.
+ * 2^(s - 127).  bf16 holds every value that an append writes; fp16 those of rows appended
+ * as fp16.
  */
 #ifndef SSATTN_PAGED8_H
 #define SSATTN_PAGED8_H
@@ -71,8 +72,10 @@ int ssa_paged8_attention(const void* q, long long q_token_stride, long long q_he
  *   window > 0:   of its own sequence a query sees the rows j > lengths[b] - n + i -
  *                 window only.  Pages that no query sees may be absent, their rows
  *                 anything.
- * 0 <= cap <= 65536, 0 <= window < 2^30; slopes are finite.  A score is off by up to 2^-22
- * of the cap. */
+ * 0 <= cap <= 65536 (and large enough that 2 log2(e) scale / cap is a finite float), 0 <=
+ * window < 2^30; slopes are finite, and so are they times the distances as floats.  A score
+ * is off by up to 2^-22 of the cap, and by up to 2^-22 of what the slope takes from it
+ * (distances beyond 2^24 are themselves rounded to floats). */
 int ssa_paged_attention_shaped(const void* q, long long q_token_stride, long long q_head_stride, const void* cache_k,
                                const void* cache_v, long long kv_token_stride, long long kv_head_stride,
                                const int32_t* prefix, int prefix_tokens, const int32_t* table, const int32_t* lengths,

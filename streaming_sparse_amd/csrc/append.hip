@@ -21,7 +21,7 @@
 // An 8-bit row is e4m3 values and one power of two: of the row as the 16-bit cache would
 // hold it, the smallest 2^e (e >= -126) with max |x| <= 448 2^e; values are rounded to
 // nearest, ties to even.  A larger mantissa than the format's would gain nothing from a
-// finer scale: its four bits are relative, and the values down to 2^-14 of the largest
+// finer scale: its four bits are relative, and the values down to 2^-13 of the largest
 // keep all of them.  With powers of two the way back is exact.
 #include "common.h"
 #include "../../include/ssattn_paged.h"
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(AppendParams p) {
   const int partner = (lane & 48) | ((second ? c - half_lanes : c + half_lanes) & 15);
   // 8-bit keys turn in float64: a step of theirs is a sixteenth of a value, and so is what
   // a rounding to the other side of a border costs, which float32 does to one value in
-  // 10^5 (36864 tokens x 36 rows 102 and 108 us)
+  // 10^5 (36864 tokens x 36 rows 102.3 and 104.1 us, ragged 7839 x 36, fp16, 24.4 and 28.2)
   float C[kNeed], S[kNeed];
   double C64[EIGHT ? kNeed : 1], S64[EIGHT ? kNeed : 1];
   if (EIGHT && has_keys) {

@@ -443,7 +443,7 @@ __device__ __forceinline__ Sight sight_of(const PagedParams& p, const Job& j, in
 
 // Products q.k into scores in log2 units: cap tanh(s / cap), s = scale q.k, as cap - 2
 // cap / (1 + e^(2 s / cap)) (its error is at most 2^-22 of the cap), less slope *
-// |distance|.  `place`: that of key 0, the prefix counted.
+// |distance| (2^-22 of that product).  `place`: that of key 0, the prefix counted.
 template <class Key>
 __device__ __forceinline__ void shape(const PagedParams& p, f32x16& S, const Sight& x, int place, Key key) {
   if (p.cap_log2 > 0.0f) {
@@ -691,9 +691,10 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
 // of 2^-17 of the largest beside values of E - 15 went missing, 3% of an output.  From
 // the first page on that has other exponents pages meet two bf16 parts in units of 1, in
 // a loop of its own (as a branch in a wide tile's first one it took its registers: 64 x 1
-// token behind 16384 127 us).  64 x 1 behind 16384 42.2 us, by two bf16 parts 46.7; 16 x
-// 1 behind 131001 77 and 85; 64 x 1 behind 64, up to 2000 own rows, 33 and 36.5.  Waves
-// by themselves, which wait for their pages, keep the two parts: a second loop beside the
+// token behind 16384 127 us).  64 x 1 behind 16384 41.4 us, by two bf16 parts (BOTH)
+// 45.7, and 50.1 where every list's first page has such exponents; 16 x 1 behind 131001
+// 77, 85 and 85; 64 x 1 behind 64, up to 2000 own rows, 33.6, 36.1 and 36.5.  Waves by
+// themselves, which wait for their pages, keep the two parts: a second loop beside the
 // prefix tiles' costs more than it saves (4 x 1, 12 heads, behind 2000 12.7 and 11.9).
 constexpr int kUnitLow = 127 - 40, kUnitHigh = 127 + 40, kUnitSpan = 15;      // as floats' exponents
 

@@ -257,10 +257,12 @@ def attention(q, cache_k, cache_v, prefix, prefix_tokens, table, lengths, worksp
     and fp16 values within 2^-11 of the type's largest, may come out infinite.
 
     Shaped scores, each for itself or together, of s = scale q.k:
-    cap (up to 65536): s becomes cap tanh(s / cap), within 2^-22 of the cap;
+    cap (up to 65536, not so small that 2 log2(e) scale / cap overflows float32): s
+    becomes cap tanh(s / cap), within 2^-22 of the cap;
     slopes [H] float32, finite: s falls by the head's slope times the distance in rows
     between query and key, query i's own row being lengths[b] - n + i and the
-    prefix's rows lying before row 0 (keys behind the query count alike);
+    prefix's rows lying before row 0 (keys behind the query count alike), within
+    2^-22 of the fall, which must be finite in float32;
     window (1 or more): of its own sequence a query sees only the `window` rows up
     to its own (without `causal` also those behind it), and all of the prefix.
     Pages that no query sees any more may be absent, and are not walked."""
