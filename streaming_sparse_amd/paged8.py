@@ -81,7 +81,7 @@ def append(k, v, cache, table, held, *, q=None, q_out=None, starts=None, freqs=N
     pages, g, where = _cache(cache, k.get_device())
     q = _append("ssa_paged8_append", where, pages, g, k, v, table, held, q, q_out, starts, freqs, axes, positions,
                 first, interleaved, workspace, code)
-    if not code:
+    if not code and k.shape[0]:
         cache.bf16 = True
     return q
 

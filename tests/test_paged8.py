@@ -190,6 +190,8 @@ def test_half_queries_over_bfloat16_rows_are_refused(no_launch):
 
     cache = a['cache']
     attend(a, cache), attend(b, cache)                        # nothing is known of its rows
+    paged8.append(a['k'][:0], a['v'][:0], cache, a['table'], a['held'])
+    attend(b, cache)                                          # and no row is none
     paged8.append(b['k'], b['v'], cache, b['table'], b['held'])
     attend(a, cache), attend(b, cache)
     paged8.append(a['k'], a['v'], cache, a['table'], a['held'])
